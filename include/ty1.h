@@ -272,6 +272,73 @@ int ty1_adam_step_f32(float *p, const float *g, float *m, float *v, int64_t n, f
                       float beta2, float eps, int64_t t, ty1_stream_t stream);
 
 /*
+ * Low-rank adapters of many requests beside the shared Dense layer (the only trainable layer, models/model_tiny_yolov1.py:96):
+ * one batch holds images of many cameras or customers, each with its own rank-R change of the Dense weight.  No counterpart in
+ * the reference, which has one set of weights.  For row n with adapter i = index[n]:
+ *   h[n][r]   = sum_k x[n][k] A[i][r][k]
+ *   out[n][u] = scale[i] * sum_r h[n][r] B[i][r][u]              (accumulate != 0: added to what out holds)
+ *   index[n] < 0: no adapter (out[n] = 0, or left as it is with accumulate; h[n] = 0).
+ *   index[n] >= L: out[n] and h[n] become NaN.
+ * x (N,K); a (L,R,K); b (L,R,U): element (i,r,c) of a at a + i*sa + r*lda + c, of b at b + i*sb + r*ldb + c, row n of x at
+ * x + n*ldx (strides in elements; the last axis is dense).  _f32: x, a, b float32.  _bf16: x, a, b bf16.  index (N) int32,
+ * scale (L) f32, out (N,U) f32 with row stride ldo, h (N,R) f32 or NULL: kept for the backward pass (without scale).  All
+ * sums are float32.  1 <= R <= 128, 1 <= L <= 4096, any N, K, U; a smaller rank is padded with zero rows of A and B.
+ * workspace: scratch of ty1_adapter_workspace_bytes() bytes, 16-byte aligned, for this call alone.  Laid out as one more split of ty1_dense_splitk_f32's partials, out is summed by whatever kernel reduces those.
+ */
+int ty1_adapter_workspace_bytes(int N, int K, int U, int L, int R, int backward, size_t *bytes);
+int ty1_adapter_forward_f32(const float *x, const float *a, const float *b, const int32_t *index, const float *scale,
+                            float *out, float *h, int N, int K, int U, int L, int R, int64_t ldx, int64_t lda, int64_t sa,
+                            int64_t ldb, int64_t sb, int64_t ldo, int accumulate, void *workspace, size_t workspace_bytes,
+                            ty1_stream_t stream);
+int ty1_adapter_forward_bf16(const void *x, const void *a, const void *b, const int32_t *index, const float *scale,
+                             float *out, float *h, int N, int K, int U, int L, int R, int64_t ldx, int64_t lda, int64_t sa,
+                             int64_t ldb, int64_t sb, int64_t ldo, int accumulate, void *workspace, size_t workspace_bytes,
+                             ty1_stream_t stream);
+/*
+ * Its gradients from dz (N,U) f32 = dL/dout (for the detector: what ty1_train_tail_f32 writes):
+ *   g[n][r]     = scale[i] * sum_u dz[n][u] B[i][r][u]
+ *   da[i][r][k] = sum over rows n with index[n] = i of g[n][r] x[n][k]
+ *   db[i][r][u] = scale[i] * sum over those rows of h[n][r] dz[n][u]
+ *   dx[n][k]    = sum_r g[n][r] A[i][r][k]                        (dx NULL: not computed)
+ * da (L,R,K), db (L,R,U), dx (N,K) are f32 and written whole: an adapter without rows gets zeros, a row without an adapter a
+ * zero dx row, a row with index >= L a NaN dx row and no part in da and db.  h as ty1_adapter_forward_* stored it, or NULL:
+ * computed again.  Rows of an adapter are summed in ascending order of n: the same bits every time.
+ */
+int ty1_adapter_backward_f32(const float *dz, const float *x, const float *a, const float *b, const int32_t *index,
+                             const float *scale, const float *h, float *da, float *db, float *dx, int N, int K, int U, int L,
+                             int R, int64_t lddz, int64_t ldx, int64_t lda, int64_t sa, int64_t ldb, int64_t sb, int64_t ldda,
+                             int64_t sda, int64_t lddb, int64_t sdb, int64_t lddx, void *workspace, size_t workspace_bytes,
+                             ty1_stream_t stream);
+int ty1_adapter_backward_bf16(const float *dz, const void *x, const void *a, const void *b, const int32_t *index,
+                              const float *scale, const float *h, float *da, float *db, float *dx, int N, int K, int U, int L,
+                              int R, int64_t lddz, int64_t ldx, int64_t lda, int64_t sa, int64_t ldb, int64_t sb, int64_t ldda,
+                              int64_t sda, int64_t lddb, int64_t sdb, int64_t lddx, void *workspace, size_t workspace_bytes,
+                              ty1_stream_t stream);
+
+/*
+ * The global norm over many gradient tensors, clipping by it, and the Adam step that clips on the way (Keras optimizers'
+ * global_clipnorm; the reference trains without clipping, train.py:59).
+ *   norm = sqrt(sum over all tensors and values of g^2), squares and sums in float64
+ *   c = 1 where norm <= max_norm, max_norm / norm above it, NaN where the norm is not finite (as tf.clip_by_global_norm)
+ *   ty1_clip_grad_norm: outs[t][j] = grads[t][j] * c, rounded to the tensor's type; outs[t] may be grads[t]
+ *   ty1_adam_step_clip_f32: ty1_adam_step_f32's step with grads[t][j] * c for the gradient; g is not written
+ * grads, outs, p, g, m, v, counts and dtypes are HOST arrays of n entries: device pointers (aligned to their type), numbers
+ * of values, and TY1_F32 or TY1_BF16 (dtypes NULL: all float32).  norm (1) f32 on the device.  Nothing of the host arrays is
+ * read after the call returns.  A tensor that is written must not overlap any other tensor of the call, except outs[t] with
+ * grads[t] of the same t and address (refused).  max_norm > 0, infinity included.  1 - beta1, 1 - beta2 and the bias-corrected
+ * rate are taken in float64 and rounded once.
+ */
+enum { TY1_F32 = 0, TY1_BF16 = 1 };
+int ty1_grad_norm_workspace_bytes(int n, size_t *bytes);
+int ty1_grad_norm(void *const *grads, const int64_t *counts, const int *dtypes, int n, float *norm, void *workspace,
+                  size_t workspace_bytes, ty1_stream_t stream);
+int ty1_clip_grad_norm(void *const *grads, void *const *outs, const int64_t *counts, const int *dtypes, int n, double max_norm,
+                       float *norm, void *workspace, size_t workspace_bytes, ty1_stream_t stream);
+int ty1_adam_step_clip_f32(void *const *p, void *const *g, void *const *m, void *const *v, const int64_t *counts, int n,
+                           double max_norm, double lr, double beta1, double beta2, double eps, int64_t t, float *norm,
+                           void *workspace, size_t workspace_bytes, ty1_stream_t stream);
+
+/*
  * The first two blocks of the bf16 network in one launch - convolution_0 and convolution_1 with their BatchNormalization,
  * LeakyReLU and MaxPooling2D layers (/root/reference/models/model_tiny_yolov1.py:43-53) - so that the (H/2, W/2, 16) tensor
  * between them stays in LDS instead of crossing HBM twice:

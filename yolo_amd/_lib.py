@@ -40,6 +40,15 @@ SIGNATURES = {
     'ty1_train_tail_f32': [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp],
     'ty1_dense_wgrad_f32': [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
     'ty1_adam_step_f32': [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _i64, _vp],
+    'ty1_adapter_workspace_bytes': [_i, _i, _i, _i, _i, _i, _vp],
+    'ty1_adapter_forward_f32': [_vp] * 7 + [_i] * 5 + [_i64] * 6 + [_i, _vp, _c.c_size_t, _vp],
+    'ty1_adapter_forward_bf16': [_vp] * 7 + [_i] * 5 + [_i64] * 6 + [_i, _vp, _c.c_size_t, _vp],
+    'ty1_adapter_backward_f32': [_vp] * 10 + [_i] * 5 + [_i64] * 11 + [_vp, _c.c_size_t, _vp],
+    'ty1_adapter_backward_bf16': [_vp] * 10 + [_i] * 5 + [_i64] * 11 + [_vp, _c.c_size_t, _vp],
+    'ty1_grad_norm_workspace_bytes': [_i, _vp],
+    'ty1_grad_norm': [_vp, _vp, _vp, _i, _vp, _vp, _c.c_size_t, _vp],
+    'ty1_clip_grad_norm': [_vp, _vp, _vp, _vp, _i, _d, _vp, _vp, _c.c_size_t, _vp],
+    'ty1_adam_step_clip_f32': [_vp, _vp, _vp, _vp, _vp, _i, _d, _d, _d, _d, _d, _i64, _vp, _vp, _c.c_size_t, _vp],
     'ty1_set_reserved_cus': [_i],
     'ty1_get_reserved_cus': [_c.POINTER(_i)],
     'ty1_prof_enable': [_i],

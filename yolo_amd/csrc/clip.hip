@@ -1,0 +1,252 @@
+// The global norm over many gradient tensors, clipping by it, and the Adam step that clips on the way.
+//
+//   norm = sqrt(sum over all tensors and values of g^2);  c = 1 if norm <= max_norm, max_norm / norm above it, NaN if not finite
+//   clip: out = g c                       (tf.clip_by_global_norm, which Keras' optimizers call for global_clipnorm)
+//   Adam: the step of train.hip on g c    (Keras semantics)
+//
+// Squares and sums are float64: the largest float32 squared is 1e77, so no finite gradient overflows and none underflows, and the
+// order of the sum is fixed by the sizes alone.  c stays float64 up to the product with g: max_norm / norm can lie below
+// float32's range.  All launches are bound by HBM: g is read once for the norm and once more by
+// what applies it.
+//
+// The tensors' addresses and lengths travel by value in the launch's arguments (no copy to the device, nothing to keep alive,
+// safe to capture); a launch takes up to kTensors of them, longer lists take several.  Seen as one concatenation, the values
+// are split evenly over the workgroups whatever the tensors' sizes are.
+#include "common.h"
+#include <algorithm>
+#include <cmath>
+
+namespace {
+
+typedef __bf16 bf16;
+
+constexpr int kTensors = 64;
+constexpr int kThreads = 256;
+
+struct Lists {
+    void *a[kTensors], *b[kTensors], *c[kTensors], *d[kTensors];   // norm: g; clip: g, out; Adam: p, g, m, v
+    long long start[kTensors + 1];                                 // values before tensor t in this launch
+    unsigned long long half;                                       // bit t: tensor t holds bf16
+    int n;
+};
+
+__device__ inline double block_sum(double v, double *lds) {
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double sum = 0.0;
+    for (int w = 0; w < (int)blockDim.x >> 6; ++w) sum += lds[w];
+    return sum;
+}
+
+// calls f(t, lo, hi) for every tensor that has values in this workgroup's share of the concatenation
+template <class F>
+__device__ inline void my_share(const Lists &ls, const F &f) {
+    const long long total = ls.start[ls.n], per = (total + gridDim.x - 1) / gridDim.x;
+    const long long lo = per * blockIdx.x, hi = lo + per < total ? lo + per : total;
+    for (int t = 0; t < ls.n; ++t) {
+        const long long a = lo > ls.start[t] ? lo : ls.start[t], b = hi < ls.start[t + 1] ? hi : ls.start[t + 1];
+        if (a < b) f(t, a - ls.start[t], b - ls.start[t]);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const Lists ls, double *__restrict__ part) {
+    __shared__ double lds[4];
+    double sum = 0.0;
+    my_share(ls, [&](int t, long long lo, long long hi) {
+        for (long long j = lo + threadIdx.x; j < hi; j += kThreads) {
+            const double v = ls.half >> t & 1 ? (double)(float)((const bf16 *)ls.a[t])[j] : (double)((const float *)ls.a[t])[j];
+            sum += v * v;
+        }
+    });
+    sum = block_sum(sum, lds);
+    if (threadIdx.x == 0) part[blockIdx.x] = sum;
+}
+
+// the norm and the coefficient from the partial sums; workgroup 0 also stores the norm
+__device__ inline double coefficient(const double *__restrict__ part, int parts, double max_norm, float *norm, double *lds) {
+    double sum = 0.0;
+    for (int j = threadIdx.x; j < parts; j += blockDim.x) sum += part[j];
+    const double n = sqrt(block_sum(sum, lds));
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
+    if (!(n < __builtin_huge_val())) return __builtin_nan("");
+    return n <= max_norm ? 1.0 : max_norm / n;
+}
+
+__global__ __launch_bounds__(kThreads) void norm_finish_kernel(const double *__restrict__ part, int parts, float *norm) {
+    __shared__ double lds[4];
+    coefficient(part, parts, 0.0, norm, lds);
+}
+
+__global__ __launch_bounds__(kThreads) void clip_kernel(const Lists ls, const double *__restrict__ part, int parts, double max_norm,
+                                                        float *norm) {
+    __shared__ double lds[4];
+    const double c = coefficient(part, parts, max_norm, norm, lds);
+    my_share(ls, [&](int t, long long lo, long long hi) {
+        for (long long j = lo + threadIdx.x; j < hi; j += kThreads)
+            if (ls.half >> t & 1) ((bf16 *)ls.b[t])[j] = (bf16)(float)((double)(float)((const bf16 *)ls.a[t])[j] * c);
+            else ((float *)ls.b[t])[j] = (float)((double)((const float *)ls.a[t])[j] * c);
+    });
+}
+
+__global__ __launch_bounds__(kThreads) void adam_clip_kernel(const Lists ls, const double *__restrict__ part, int parts,
+                                                             double max_norm, float *norm, float lr_t, float b1, float b2, float c1, float c2, float eps) {
+    __shared__ double lds[4];
+    const double c = coefficient(part, parts, max_norm, norm, lds);
+    my_share(ls, [&](int t, long long lo, long long hi) {
+        float *p = (float *)ls.a[t], *m = (float *)ls.c[t], *v = (float *)ls.d[t];
+        const float *g = (const float *)ls.b[t];
+        for (long long j = lo + threadIdx.x; j < hi; j += kThreads) {
+            const float gj = (float)((double)g[j] * c);
+            const float mj = b1 * m[j] + c1 * gj, vj = b2 * v[j] + c2 * (gj * gj);
+            m[j] = mj;
+            v[j] = vj;
+            p[j] -= lr_t * mj / (sqrtf(vj) + eps);
+        }
+    });
+}
+
+int blocks_for(long long total) {
+    const long long want = (total + 4095) / 4096, most = 4ll * ty1::num_cus();
+    return (int)(want < 1 ? 1 : want > most ? most : want);
+}
+
+// No tensor that is written may share memory with another one (a value scaled twice, or read after it was scaled): all address
+// ranges in order, each against the ranges that reach furthest before it.  Bit l of `written`: list l is written; list 1 may
+// lie exactly on list 0 where `in_place`.
+int check_overlap(const char *what, int n, const int64_t *counts, const int *dtypes, void *const *const *lists, int n_lists,
+                  unsigned written, bool in_place) {
+    struct Range {
+        uintptr_t lo, hi;
+        int t;
+        bool w;
+    };
+    Range *r = (Range *)malloc(sizeof(Range) * (size_t)n * n_lists);
+    TY1_REQUIRE(r, "%s: out of host memory", what);
+    size_t k = 0;
+    for (int l = 0; l < n_lists; ++l)
+        for (int t = 0; t < n; ++t) {
+            if (counts[t] == 0 || (in_place && l == 0 && lists[1][t] == lists[0][t])) continue;
+            const uintptr_t lo = (uintptr_t)lists[l][t];
+            r[k++] = {lo, lo + (uintptr_t)counts[t] * (dtypes && dtypes[t] == TY1_BF16 ? 2 : 4), t, (written >> l & 1) != 0};
+        }
+    std::sort(r, r + k, [](const Range &a, const Range &b) { return a.lo < b.lo; });
+    uintptr_t read_to = 0, written_to = 0;
+    int bad = -1;
+    for (size_t j = 0; j < k && bad < 0; ++j) {
+        if (r[j].lo < written_to || (r[j].w && r[j].lo < read_to)) bad = r[j].t;
+        uintptr_t &to = r[j].w ? written_to : read_to;
+        if (r[j].hi > to) to = r[j].hi;
+    }
+    free(r);
+    TY1_REQUIRE(bad < 0, "%s: tensor %d shares memory with another tensor of the call", what, bad);
+    return 0;
+}
+
+// lists of n host pointers: element sizes and addresses have to fit
+int check_lists(const char *what, int n, const int64_t *counts, const int *dtypes, void *const *const *lists, int n_lists) {
+    TY1_REQUIRE(n >= 1 && counts, "%s: no tensors", what);
+    for (int l = 0; l < n_lists; ++l) TY1_REQUIRE(lists[l], "%s: null list", what);
+    for (int t = 0; t < n; ++t) {
+        TY1_REQUIRE(counts[t] >= 0, "%s: tensor %d has %lld values", what, t, (long long)counts[t]);
+        TY1_REQUIRE(!dtypes || dtypes[t] == TY1_F32 || dtypes[t] == TY1_BF16, "%s: tensor %d has type %d", what, t, dtypes[t]);
+        const uintptr_t align = dtypes && dtypes[t] == TY1_BF16 ? 2 : 4;
+        for (int l = 0; l < n_lists; ++l)
+            TY1_REQUIRE(counts[t] == 0 || (lists[l][t] && ((uintptr_t)lists[l][t] & (align - 1)) == 0), "%s: tensor %d: null or misaligned pointer", what, t);
+    }
+    return 0;
+}
+
+// fills ls with tensors t0, t0 + 1, ... -> how many list entries were consumed
+int fill(Lists &ls, int t0, int n, const int64_t *counts, const int *dtypes, void *const *const *lists, int n_lists) {
+    ls.n = 0;
+    ls.half = 0;
+    ls.start[0] = 0;
+    int t = t0;
+    for (; t < n && ls.n < kTensors; ++t) {
+        if (counts[t] == 0) continue;
+        void **dst[4] = {ls.a, ls.b, ls.c, ls.d};
+        for (int l = 0; l < n_lists; ++l) dst[l][ls.n] = lists[l][t];
+        if (dtypes && dtypes[t] == TY1_BF16) ls.half |= 1ull << ls.n;
+        ls.start[ls.n + 1] = ls.start[ls.n] + counts[t];
+        ++ls.n;
+    }
+    return t - t0;
+}
+
+size_t partials(int n) { return (size_t)((n + kTensors - 1) / kTensors) * 4 * ty1::num_cus(); }
+
+// the squares of list `which`, launch by launch -> number of partial sums in ws
+int launch_norm(int n, const int64_t *counts, const int *dtypes, void *const *list, double *part, hipStream_t s) {
+    int parts = 0;
+    Lists ls;
+    for (int t = 0; t < n;) {
+        t += fill(ls, t, n, counts, dtypes, &list, 1);
+        if (ls.n == 0) break;
+        const int blocks = blocks_for(ls.start[ls.n]);
+        norm_kernel<<<dim3(blocks), dim3(kThreads), 0, s>>>(ls, part + parts);
+        parts += blocks;
+    }
+    return parts;
+}
+
+}  // namespace
+
+extern "C" int ty1_grad_norm_workspace_bytes(int n, size_t *bytes) {
+    TY1_REQUIRE(bytes && n >= 1, "ty1_grad_norm_workspace_bytes: bad arguments");
+    *bytes = partials(n) * sizeof(double);
+    return 0;
+}
+
+extern "C" int ty1_grad_norm(void *const *grads, const int64_t *counts, const int *dtypes, int n, float *norm, void *workspace,
+                             size_t workspace_bytes, ty1_stream_t stream) {
+    if (check_lists("ty1_grad_norm", n, counts, dtypes, &grads, 1)) return 1;
+    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_grad_norm: null pointer or workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    ty1::ProfScope prof("grad_norm", s);
+    const int parts = launch_norm(n, counts, dtypes, grads, (double *)workspace, s);
+    norm_finish_kernel<<<dim3(1), dim3(kThreads), 0, s>>>((const double *)workspace, parts, norm);
+    return ty1::check_launch("ty1_grad_norm");
+}
+
+extern "C" int ty1_clip_grad_norm(void *const *grads, void *const *outs, const int64_t *counts, const int *dtypes, int n,
+                                  double max_norm, float *norm, void *workspace, size_t workspace_bytes, ty1_stream_t stream) {
+    void *const *lists[2] = {grads, outs};
+    if (check_lists("ty1_clip_grad_norm", n, counts, dtypes, lists, 2) || check_overlap("ty1_clip_grad_norm", n, counts, dtypes, lists, 2, 2u, true)) return 1;
+    TY1_REQUIRE(max_norm > 0.0, "ty1_clip_grad_norm: max_norm=%g must be positive", max_norm);
+    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_clip_grad_norm: null pointer or workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    ty1::ProfScope prof("clip_grad_norm", s);
+    const int parts = launch_norm(n, counts, dtypes, grads, (double *)workspace, s);
+    Lists ls;
+    int t = 0;
+    do {
+        t += fill(ls, t, n, counts, dtypes, lists, 2);
+        clip_kernel<<<dim3(blocks_for(ls.start[ls.n])), dim3(kThreads), 0, s>>>(ls, (const double *)workspace, parts, max_norm, norm);
+    } while (t < n);
+    return ty1::check_launch("ty1_clip_grad_norm");
+}
+
+extern "C" int ty1_adam_step_clip_f32(void *const *p, void *const *g, void *const *m, void *const *v, const int64_t *counts, int n,
+                                      double max_norm, double lr, double beta1, double beta2, double eps, int64_t t, float *norm,
+                                      void *workspace, size_t workspace_bytes, ty1_stream_t stream) {
+    void *const *lists[4] = {p, g, m, v};
+    if (check_lists("ty1_adam_step_clip", n, counts, nullptr, lists, 4) || check_overlap("ty1_adam_step_clip", n, counts, nullptr, lists, 4, 13u, false)) return 1;
+    TY1_REQUIRE(max_norm > 0.0, "ty1_adam_step_clip: max_norm=%g must be positive", max_norm);
+    TY1_REQUIRE(t >= 1, "ty1_adam_step_clip: bad t=%lld", (long long)t);
+    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_adam_step_clip: null pointer or workspace too small");
+    const double lr_t = lr * std::sqrt(1.0 - std::pow(beta2, (double)t)) / (1.0 - std::pow(beta1, (double)t));
+    hipStream_t s = (hipStream_t)stream;
+    ty1::ProfScope prof("adam_step_clip", s);
+    const int parts = launch_norm(n, counts, nullptr, g, (double *)workspace, s);
+    Lists ls;
+    int k = 0;
+    do {
+        k += fill(ls, k, n, counts, nullptr, lists, 4);
+        adam_clip_kernel<<<dim3(blocks_for(ls.start[ls.n])), dim3(kThreads), 0, s>>>(ls, (const double *)workspace, parts, max_norm, norm,
+                                                                                    (float)lr_t, (float)beta1, (float)beta2, (float)(1.0 - beta1),
+                                                                                    (float)(1.0 - beta2), (float)eps);
+    } while (k < n);
+    return ty1::check_launch("ty1_adam_step_clip_f32");
+}

@@ -1,5 +1,7 @@
 """Thin host wrappers: torch ROCm tensors are used only as device buffers; every op below is one
 call into libty1.so (hand-written gfx950 kernels) on the current torch stream."""
+import ctypes
+
 import torch
 
 from . import _lib
@@ -458,6 +460,227 @@ def adam_step(p, g, m, v, t, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7):
         _chk(a, torch.float32, name)
     _lib.call('ty1_adam_step_f32', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
               float(lr), float(beta1), float(beta2), float(eps), int(t), _lib.current_stream())
+
+
+# ------------------------------------------------------------------ low-rank adapters, gradient clipping
+MAX_RANK, MAX_ADAPTERS = 128, 4096          # of ty1_adapter_*
+
+
+def _call_on(index, name, *args):
+    """The call on device `index` and its current torch stream: the tensors' device, whatever the current one is."""
+    if index == torch.cuda.current_device():
+        return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+
+
+def _strided(t, dtype, shape, index, name):
+    """A tensor on device `index` with a dense last axis and any strides in front of it."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        raise TypeError(f'{name}: expected a tensor on GPU {index}')
+    if t.dtype != dtype:
+        raise TypeError(f'{name}: expected {dtype}, got {t.dtype}')
+    if t.shape != shape:
+        raise ValueError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f'{name}: the last axis must be dense, its stride is {t.stride(-1)}')
+    return t
+
+
+def _span(t):
+    """First and last address + 1 of a tensor's values."""
+    lo = t.data_ptr()
+    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else lo
+
+
+def _chk_written(outs, ins):
+    """Outputs that the caller brings: rows that do not overlap one another, and memory apart from the operands'."""
+    for name, t in outs:
+        st, n = t.stride(), t.shape
+        need = n[-1]
+        for d in range(t.dim() - 2, -1, -1):
+            if n[d] > 1 and st[d] < need:
+                raise ValueError(f'{name}: strides {st} make its rows overlap')
+            need = st[d] * (n[d] - 1) + need
+    spans = [(name, *_span(t)) for name, t in list(outs) + list(ins)]
+    for i in range(len(outs)):
+        for j in range(i + 1, len(spans)):
+            if spans[i][1] < spans[j][2] and spans[j][1] < spans[i][2]:
+                raise ValueError(f'{spans[i][0]}: shares memory with {spans[j][0]}')
+
+
+def _adapter_operands(x, a, b, index, scale):
+    """Checks the operands both passes share -> (device index, N, K, U, L, R)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise TypeError('x: expected a tensor on the GPU (ROCm device)')
+    if x.dtype is not torch.float32 and x.dtype is not torch.bfloat16:
+        raise TypeError(f'x: expected torch.float32 or torch.bfloat16, got {x.dtype}')
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError(f'expected x (N,K), a (L,R,K), b (L,R,U), got {tuple(x.shape)}, {tuple(a.shape)}, {tuple(b.shape)}')
+    dev = x.get_device()
+    N, K = x.shape
+    L, R, U = b.shape
+    if not (1 <= R <= MAX_RANK and 1 <= L <= MAX_ADAPTERS):
+        raise ValueError(f'{L} adapters of rank {R}: 1 to {MAX_ADAPTERS} of rank 1 to {MAX_RANK} are supported')
+    if K < 1 or U < 1 or max(N, K, U) >= 2 ** 31:
+        raise ValueError(f'x (N,K) = {(N, K)}, b (L,R,U) = {(L, R, U)}: sizes must be positive (N may be 0) and below 2^31')
+    _strided(x, x.dtype, (N, K), dev, 'x'); _strided(a, x.dtype, (L, R, K), dev, 'a'); _strided(b, x.dtype, (L, R, U), dev, 'b')
+    _strided(index, torch.int32, (N,), dev, 'index'); _strided(scale, torch.float32, (L,), dev, 'scale')
+    return dev, N, K, U, L, R
+
+
+def _adapter_workspace(x, N, K, U, L, R, backward):
+    size = ctypes.c_size_t(0)
+    _lib.call('ty1_adapter_workspace_bytes', N, K, U, L, R, backward, ctypes.addressof(size))
+    return torch.empty((size.value,), dtype=torch.uint8, device=x.device)
+
+
+def adapter_forward(x, a, b, index, scale, out=None, accumulate=False, h=None):
+    """The low-rank adapters of many requests in one batch, beside the Dense layer that they share:
+        out[n] = scale[i] * (x[n] . a[i]^T) . b[i],   i = index[n]
+    x (N,K), a (L,R,K), b (L,R,U): all float32 or all bfloat16, last axis dense, any strides in front of it (a row of x may be
+    repeated by expand); index (N) int32; scale (L) float32 -> out (N,U) float32, sums in float32.
+    index[n] < 0: no adapter for this row (zeros).  index[n] >= L: the row becomes NaN (the index lives on the GPU and is not
+    read by the host).  Smaller ranks: zero rows in a and b.
+    out: where to write, e.g. part[splits][:, :U] behind the partials of dense_splitk - the kernel that reduces those then adds
+    the adapters at no cost.  accumulate: add to what out holds instead (rows without an adapter stay as they are).
+    h: optional (N,R) float32 that receives x . a^T (without scale) for adapter_backward."""
+    dev, N, K, U, L, R = _adapter_operands(x, a, b, index, scale)
+    if out is None:
+        if accumulate:
+            raise ValueError('accumulate needs out')
+        out = torch.empty((N, U), dtype=torch.float32, device=x.device)
+        if h is not None:
+            _chk_written([('h', _chk_out(h, torch.float32, (N, R), 'h'))], [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
+    else:
+        outs = [('out', _strided(out, torch.float32, (N, U), dev, 'out'))]
+        if h is not None:
+            outs.append(('h', _chk_out(h, torch.float32, (N, R), 'h')))
+        _chk_written(outs, [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
+    if N == 0:
+        return out
+    ws = _adapter_workspace(x, N, K, U, L, R, 0)
+    _call_on(dev, 'ty1_adapter_forward_bf16' if x.dtype is torch.bfloat16 else 'ty1_adapter_forward_f32', x.data_ptr(), a.data_ptr(),
+             b.data_ptr(), index.data_ptr(), scale.data_ptr(), out.data_ptr(), _lib.ptr(h), N, K, U, L, R, x.stride(0), a.stride(1),
+             a.stride(0), b.stride(1), b.stride(0), out.stride(0), int(bool(accumulate)), ws.data_ptr(), ws.numel())
+    return out
+
+
+def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, db=None, dx=None):
+    """Gradients of adapter_forward from dz (N,U) float32 = dL/dout -> (da (L,R,K), db (L,R,U), dx (N,K) or None), float32.
+    h: what adapter_forward stored, or None: computed again.  da, db, dx: optional buffers; they are written whole (zeros for
+    an adapter without rows, for a dx row without an adapter; NaN for the dx row of an index >= L).  want_dx: also the
+    gradient of x (the detector's backbone is frozen and needs none); giving dx asks for it too.
+    The rows of an adapter are summed in a fixed order: the same bits every time."""
+    dev, N, K, U, L, R = _adapter_operands(x, a, b, index, scale)
+    _strided(dz, torch.float32, (N, U), dev, 'dz')
+    if h is not None:
+        _chk_out(_strided(h, torch.float32, (N, R), dev, 'h'), torch.float32, (N, R), 'h')
+    given = [(name, _strided(t, torch.float32, shape, dev, name)) for name, t, shape in
+             (('da', da, (L, R, K)), ('db', db, (L, R, U)), ('dx', dx, (N, K))) if t is not None]
+    if given:
+        _chk_written(given, [('dz', dz), ('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)] + ([('h', h)] if h is not None else []))
+    da = torch.empty((L, R, K), dtype=torch.float32, device=x.device) if da is None else da
+    db = torch.empty((L, R, U), dtype=torch.float32, device=x.device) if db is None else db
+    if dx is None and want_dx:
+        dx = torch.empty((N, K), dtype=torch.float32, device=x.device)
+    ws = _adapter_workspace(x, N, K, U, L, R, 1)
+    _call_on(dev, 'ty1_adapter_backward_bf16' if x.dtype is torch.bfloat16 else 'ty1_adapter_backward_f32', dz.data_ptr(), x.data_ptr(),
+             a.data_ptr(), b.data_ptr(), index.data_ptr(), scale.data_ptr(), _lib.ptr(h), da.data_ptr(), db.data_ptr(), _lib.ptr(dx),
+             N, K, U, L, R, dz.stride(0), x.stride(0), a.stride(1), a.stride(0), b.stride(1), b.stride(0), da.stride(1), da.stride(0),
+             db.stride(1), db.stride(0), dx.stride(0) if dx is not None else 0, ws.data_ptr(), ws.numel())
+    return da, db, dx
+
+
+def _tensor_lists(**lists):
+    """One tensor or equally long lists of contiguous tensors on one GPU, float32 or bfloat16 -> (device index, n, the lists'
+    pointer arrays, value counts, types): the HOST arrays of ty1_grad_norm and its kin."""
+    names, first = list(lists), None
+    arrays = []
+    for name, ts in lists.items():
+        ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
+        lists[name] = ts
+        if first is None:
+            first = ts
+            if not ts:
+                raise ValueError(f'{name}: no tensors')
+            for t in ts:
+                if not isinstance(t, torch.Tensor):
+                    raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
+            dev, dtypes, counts = ts[0].get_device(), [t.dtype for t in ts], [t.numel() for t in ts]
+            if dev < 0:
+                raise TypeError(f'{name}: expected tensors on the GPU (ROCm device)')
+            for dt in set(dtypes):
+                if dt is not torch.float32 and dt is not torch.bfloat16:
+                    raise TypeError(f'{name}: expected torch.float32 or torch.bfloat16, got {dt}')
+        elif len(ts) != len(first):
+            raise ValueError(f'{name}: {len(ts)} tensors, {names[0]} has {len(first)}')
+        else:
+            for t, like in zip(ts, first):
+                if not isinstance(t, torch.Tensor) or t.dtype != like.dtype:
+                    raise TypeError(f'{name}: expected tensors of the types of {names[0]}')
+                if t.shape != like.shape:
+                    raise ValueError(f'{name}: expected shape {tuple(like.shape)}, got {tuple(t.shape)}')
+        for t in ts:
+            if t.get_device() != dev:
+                raise TypeError(f'{name}: all tensors must be on GPU {dev}')
+            if not t.is_contiguous():
+                raise ValueError(f'{name}: must be contiguous')
+        arrays.append((ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]))
+    n = len(first)
+    kinds = None if torch.bfloat16 not in dtypes else (ctypes.c_int * n)(*[int(dt is torch.bfloat16) for dt in dtypes])
+    return dev, n, arrays, (ctypes.c_int64 * n)(*counts), kinds
+
+
+def _norm_buffers(dev, n, norm):
+    size = ctypes.c_size_t(0)
+    _lib.call('ty1_grad_norm_workspace_bytes', n, ctypes.addressof(size))
+    device = torch.device('cuda', dev)
+    ws = torch.empty((size.value,), dtype=torch.uint8, device=device)
+    return ws, torch.empty((1,), dtype=torch.float32, device=device) if norm is None else _chk_out(norm, torch.float32, (1,), 'norm')
+
+
+def _max_norm(v):
+    v = float(v)
+    if not v > 0.0:
+        raise ValueError(f'max_norm must be positive, got {v}')
+    return v
+
+
+def grad_norm(grads, norm=None):
+    """The global 2-norm of one tensor or a list of tensors (float32 or bfloat16, contiguous, any sizes) -> (1,) float32 on
+    the device: squares and sums in float64, in an order fixed by the sizes.  norm: optional (1,) buffer."""
+    dev, n, (g,), counts, kinds = _tensor_lists(grads=grads)
+    ws, norm = _norm_buffers(dev, n, norm)
+    _call_on(dev, 'ty1_grad_norm', g, counts, kinds, n, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    return norm
+
+
+def clip_grad_norm(grads, max_norm, out=None, norm=None):
+    """Scales one tensor or a list of tensors by min(1, max_norm / global norm), in place or into out (as many tensors of the
+    same shapes and types) -> the norm before clipping, (1,) float32 on the device.  A norm that is not finite makes every
+    value NaN (Keras' global_clipnorm, tf.clip_by_global_norm).  Tensors must not overlap one another."""
+    max_norm = _max_norm(max_norm)
+    dev, n, arrays, counts, kinds = _tensor_lists(grads=grads, out=out) if out is not None else _tensor_lists(grads=grads)
+    ws, norm = _norm_buffers(dev, n, norm)
+    _call_on(dev, 'ty1_clip_grad_norm', arrays[0], arrays[-1], counts, kinds, n, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    return norm
+
+
+def adam_step_clipped(p, g, m, v, t, max_norm, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, norm=None):
+    """adam_step over one tensor or lists of float32 tensors with the gradients scaled by min(1, max_norm / global norm) on
+    the way (Keras Adam(global_clipnorm=max_norm)); g is left as it is -> the norm before clipping, (1,) float32 on the device.
+    max_norm may be infinite (no clipping).  A norm that is not finite makes the step NaN, as an unclipped one would be."""
+    max_norm = _max_norm(max_norm)
+    if int(t) < 1:
+        raise ValueError(f't is the 1-based step count, got {t}')
+    dev, n, (pp, gg, mm, vv), counts, kinds = _tensor_lists(p=p, g=g, m=m, v=v)
+    if kinds is not None:
+        raise TypeError('p, g, m, v: expected torch.float32')
+    ws, norm = _norm_buffers(dev, n, norm)
+    _call_on(dev, 'ty1_adam_step_clip_f32', pp, gg, mm, vv, counts, n, max_norm, float(lr), float(beta1), float(beta2), float(eps),
+             int(t), norm.data_ptr(), ws.data_ptr(), ws.numel())
+    return norm
 
 
 class KernelTimer:
