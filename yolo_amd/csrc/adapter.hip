@@ -10,6 +10,7 @@
 // (x.A^T and dz.B^T), expand the rank (h.B and g.A), and contract the rows of one adapter (g^T.x and h^T.dz).  All sums are
 // float32; bf16 operands are widened as they are read.
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
@@ -24,13 +25,13 @@ typedef __bf16 bf16x8_m __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 bf16x4_m __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kMaxRank = 128, kMaxAdapters = 4096;
-constexpr int kSelfPlan = 256;            // rows up to which every workgroup finds its tile by itself (one thread per row)
+constexpr int kSelfPlan = 256;            // rows up to which every workgroup finds its tile by itself
 
 // ---------------------------------------------------------------------------------------------------------------- tiles
 // The rows of a batch come in any order of adapters; a tile is up to TM rows of ONE adapter, so that the adapter's weights are
 // read once for all of them.  Rows without an adapter (index < 0 or >= L) form a class of their own, L, whose tiles are only
-// filled in.  Up to kSelfPlan rows a workgroup works its tile out from the index (below 1 us, and no launch); above, one
-// workgroup sorts the rows once (plan_kernel) and the others read the list.
+// filled in.  Up to kSelfPlan rows every workgroup works its tile out from the index itself; above, one workgroup sorts the
+// rows once (plan_kernel, 4 to 6 us and a launch) and the others read the list.
 struct Plan {
     const int *index;          // (N)
     int N, L;
@@ -42,16 +43,69 @@ struct Plan {
 
 __device__ inline int class_of(int i, int L) { return i < 0 || i >= L ? L : i; }
 
-struct alignas(16) TileLds {
-    int cls[kSelfPlan];
+struct TileLds {
     int rows[64];
-    int wave_leaders[4];
-    int adapter, first;
 };
 
-// tile t -> its class and number of rows (0: there is no tile t); lds.rows holds them.  All 256 threads call it.
-template <int TM>
-__device__ inline int find_tile(const Plan &p, int t, TileLds &lds, int &adapter) {
+// Up to 64 W rows, W to a lane: every wave finds the tile for itself by ballots over the bits of the class, without a barrier
+// (a version that compares rows through LDS took 2 to 3 us more).  A row leads a tile when the rows of its class before it are
+// a multiple of TM; tile t belongs to the t-th leader.
+template <int W>
+__device__ inline int tile_by_ballots(const Plan &p, int t, int TM, TileLds &lds, int &adapter) {
+    const int lane = threadIdx.x & 63;
+    int cls[W], before[W];
+    unsigned long long same[W][W];                     // lanes of word v with the class of this lane's row in word w >= v
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int n = 64 * w + lane;
+        cls[w] = n < p.N ? class_of(p.index[n], p.L) : p.L + 1;
+#pragma unroll
+        for (int v = 0; v <= w; ++v) same[w][v] = ~0ull;
+    }
+    for (int b = 0; (p.L + 1) >> b; ++b) {
+        unsigned long long set[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) set[w] = __ballot(cls[w] >> b & 1);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const unsigned long long all = -(unsigned long long)(cls[w] >> b & 1);
+#pragma unroll
+            for (int v = 0; v <= w; ++v) same[w][v] &= ~(set[v] ^ all);
+        }
+    }
+    const unsigned long long below = (1ull << lane) - 1;
+    int passed = 0, first = 0;
+    adapter = -1;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        before[w] = __popcll(same[w][w] & below);
+#pragma unroll
+        for (int v = 0; v < w; ++v) before[w] += __popcll(same[w][v]);
+        const bool leads = 64 * w + lane < p.N && (before[w] & (TM - 1)) == 0;
+        const unsigned long long leaders = __ballot(leads);
+        const unsigned long long mine = __ballot(leads && passed + __popcll(leaders & below) == t);
+        if (mine) {
+            const int lead = __builtin_ctzll(mine);
+            adapter = __builtin_amdgcn_readlane(cls[w], lead);
+            first = __builtin_amdgcn_readlane(before[w], lead);
+        }
+        passed += __popcll(leaders);
+    }
+    if (adapter < 0) return 0;
+    int count = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int slot = before[w] - first;
+        const bool in = cls[w] == adapter && slot >= 0 && slot < TM;
+        if (in) lds.rows[slot] = 64 * w + lane;        // all waves write the same: each reads what it wrote itself
+        count += __popcll(__ballot(in));
+    }
+    __builtin_amdgcn_wave_barrier();
+    return count;
+}
+
+// tile t of up to TM rows -> its class and number of rows (0: there is no tile t); lds.rows holds them.  All 256 threads call it.
+__device__ inline int find_tile(const Plan &p, int t, int TM, TileLds &lds, int &adapter) {
     const int tid = threadIdx.x;
     if (p.perm) {
         if (t >= *p.ntiles) return 0;
@@ -61,32 +115,9 @@ __device__ inline int find_tile(const Plan &p, int t, TileLds &lds, int &adapter
         __syncthreads();
         return tile.z;
     }
-    // a row leads a tile when the rows of its class before it are a multiple of TM; tile t belongs to the t-th leader
-    const int cls = tid < p.N ? class_of(p.index[tid], p.L) : -1;
-    lds.cls[tid] = cls;
-    if (tid == 0) lds.adapter = -1;
-    __syncthreads();
-    int before = 0;
-    for (int m = 0; m < p.N; m += 4) {
-        const int4 c = *reinterpret_cast<const int4 *>(lds.cls + m);
-        before += (c.x == cls && m < tid) + (c.y == cls && m + 1 < tid) + (c.z == cls && m + 2 < tid) + (c.w == cls && m + 3 < tid);
-    }
-    const bool leads = cls >= 0 && before % TM == 0;
-    const unsigned long long vote = __ballot(leads);
-    if ((tid & 63) == 0) lds.wave_leaders[tid >> 6] = __popcll(vote);
-    __syncthreads();
-    int place = __popcll(vote & ((1ull << (tid & 63)) - 1));
-    for (int w = 0; w < tid >> 6; ++w) place += lds.wave_leaders[w];
-    if (leads && place == t) {
-        lds.adapter = cls;
-        lds.first = before;
-    }
-    __syncthreads();
-    adapter = lds.adapter;
-    const int slot = before - lds.first;
-    const bool mine = adapter >= 0 && cls == adapter && slot >= 0 && slot < TM;
-    if (mine) lds.rows[slot] = tid;
-    return __syncthreads_count(mine);
+    if (p.N <= 64) return tile_by_ballots<1>(p, t, TM, lds, adapter);
+    if (p.N <= 128) return tile_by_ballots<2>(p, t, TM, lds, adapter);
+    return tile_by_ballots<4>(p, t, TM, lds, adapter);
 }
 
 // One workgroup sorts the rows by class (a stable counting sort, so that an adapter's rows stay in ascending order) and cuts
@@ -162,172 +193,317 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
 
 // ------------------------------------------------------------------------------------------------------------- contract
 // part[s][n][r] = sum over K slice s of x[n][k] m[i][r][k], for the rows of one tile against their adapter: a GEMM tile of
-// TM rows x R ranks, K long.  Bound by reading x and m once (both stream from memory, nothing is read twice by a tile), so the
-// operands go straight from memory into the registers of the matrix instruction: lane (j, q) of a 16-row fragment holds 16
-// consecutive bytes of row j at q * 16 bytes - four float32 steps of v_mfma_f32_16x16x4_f32 with k in another order, the same
-// on both sides, or one bf16 step of v_mfma_f32_16x16x32_bf16.  The four waves take a quarter of the slice each and join in
-// LDS; the next fragments are in flight while the present ones multiply.
-template <class TX, class TM>
+// TM rows x R ranks, K long.  Bound by reading x and m once.  A matrix fragment takes 16 bytes of each of 16 rows from
+// neighbouring lanes, which as a load from memory is 64 cache accesses an instruction (measured at 4096 rows of rank 64: the
+// cache's access rate held the kernel at 115 us); so a stage of 256 to 1024 consecutive bytes of every row goes through
+// registers into LDS, 16 accesses an instruction, and the fragments are read from there.  A row's 16-byte pieces are permuted
+// by its number: the 16 rows of a fragment read lie in 16 different bank groups.  The loads of the next stage are in flight
+// while the present one multiplies; every wave takes a quarter of a stage's K, and the four sums join in LDS.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Piece_m {               // 16 bytes from wherever a row's elements lie
+    u32x4 v;
+};
+
+template <class T>
+__device__ inline u32x4 load_piece(const T *p, int left) {          // the first `left` of a piece's elements, zeros behind them
+    constexpr int E = 16 / sizeof(T);
+    if (left >= E) return ((const Piece_m *)p)->v;
+    T e[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) e[k] = k < left ? p[k] : (T)0.f;
+    return __builtin_bit_cast(u32x4, e);
+}
+
+template <class TX, class TW>
+struct ContractArgs {
+    const TX *x;               // (N,K) stride ldx
+    const TW *m;               // (L,R,K) strides sm, ldm
+    float *part;               // (slices, N, R16): R rounded up to the tile's 16s, so that a row is whole 16-byte pieces
+    long long ldx, ldm, sm;
+    int K, R, slices;
+};
+
+// elements of K in a stage: 256 bytes a row for tall tiles, up to 1024 for low ones (two to ten loads a thread in flight)
+constexpr int stage_elements(int nt, int rt, int sx, int sw) { return (nt + rt <= 2 ? 1024 : nt + rt <= 3 || sx != sw ? 512 : 256) / sx; }
+
+// The waves' sums of a tile, (0 + 2) + (1 + 3): into red[0 .. TM R16) + red[TM R16 ..).
+template <int NB, int NT, int RT>
+__device__ inline void join_waves(const f32x4 (&acc)[NB][RT], float *red) {
+    constexpr int TM = 16 * NT, R16 = 16 * RT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, q = lane >> 4;
+    float *mine = red + (wave & 1) * TM * R16 + 4 * q * R16 + j;
+    if (wave >= 2) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mine[(16 * b + v) * R16 + 16 * r] = acc[b][r][v];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mine[(16 * b + v) * R16 + 16 * r] += acc[b][r][v];
+    }
+    __syncthreads();
+}
+
+// The direct form.  (a) fragments of a lane:
+template <class TX, class TW>
 struct Frag;
 template <>
 struct Frag<float, float> {
     typedef f32x4 VX;
     typedef f32x4 VM;
-    static constexpr int E = 4;                        // elements of a lane
-    static __device__ VX load(const float *p) { return *(const f32x4_m *)p; }
-    static __device__ f32x4 mma(const VX &a, const VM &b, f32x4 c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
-        return c;
-    }
+    static constexpr int E = 4, STEPS = 4;             // elements of a lane, matrix instructions of a fragment
+    static __device__ f32x4 mma(const VX &a, const VM &b, int e, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0); }
 };
 template <>
 struct Frag<bf16, bf16> {
     typedef bf16x8 VX;
     typedef bf16x8 VM;
-    static constexpr int E = 8;
-    static __device__ VX load(const bf16 *p) { return *(const bf16x8_m *)p; }
-    static __device__ f32x4 mma(const VX &a, const VM &b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static constexpr int E = 8, STEPS = 1;
+    static __device__ f32x4 mma(const VX &a, const VM &b, int, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Frag<float, bf16> {                             // float32 gradients against bf16 weights: widened, exact
     typedef f32x4 VX;
     typedef bf16x4 VM;
-    static constexpr int E = 4;
-    static __device__ VX load(const float *p) { return *(const f32x4_m *)p; }
-    static __device__ VM load(const bf16 *p) { return *(const bf16x4_m *)p; }
-    static __device__ f32x4 mma(const VX &a, const VM &b, f32x4 c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], (float)b[e], c, 0, 0, 0);
-        return c;
-    }
+    static constexpr int E = 4, STEPS = 4;
+    static __device__ f32x4 mma(const VX &a, const VM &b, int e, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], (float)b[e], c, 0, 0, 0); }
 };
 template <class V, class T>
-__device__ inline V load_tail(const T *p, int n, int left) {       // what there is of n elements, zeros behind
+__device__ inline V load_lane(const T *p, int left) {               // the first `left` of a lane's elements, zeros behind them
+    struct __attribute__((packed, aligned(2))) M {
+        V v;
+    };
+    constexpr int E = sizeof(V) / sizeof(T);
+    if (left >= E) return ((const M *)p)->v;
     V v;
-    for (int e = 0; e < n; ++e) v[e] = e < left ? p[e] : (T)0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < left ? p[e] : (T)0.f;
     return v;
 }
 
-template <class TX, class TM>
-struct ContractArgs {
-    const TX *x;               // (N,K) stride ldx
-    const TM *m;               // (L,R,K) strides sm, ldm
-    float *part;               // (slices, N, R)
-    long long ldx, ldm, sm;
-    int K, R, slices;
-};
-
-template <class TX, class TW, int NT, int RT>
-__global__ __launch_bounds__(256) void contract_kernel(const ContractArgs<TX, TW> a, const Plan p) {
+// (b) The waves take neighbouring groups of UN fragments in turn, so that the workgroup reads 256 consecutive bytes of a row or
+// more at a time.  UN is the same for full and partial tiles: a row's sum does not depend on the tile it is in.
+template <class TX, class TW, int NB, int NT, int RT>
+__device__ inline void contract_direct(const ContractArgs<TX, TW> &a, const int *rows, int count, int adapter, int s, float *red) {
     typedef Frag<TX, TW> F;
     typedef typename F::VX VX;
     typedef typename F::VM VM;
-    constexpr int TM = 16 * NT, R16 = 16 * RT, E = F::E, KC = 4 * E;
-    constexpr int UN = 16 / (NT + RT) < 2 ? 2 : 16 / (NT + RT) > 8 ? 8 : 16 / (NT + RT);      // fragments in flight per operand row
-    __shared__ TileLds tl;
-    __shared__ float red[4][TM * R16];
+    constexpr int R16 = 16 * RT, E = F::E, KC = 4 * E;
+    constexpr int UN = NT + RT >= 6 ? 2 : 16 / (NT + RT) > 4 ? 4 : 16 / (NT + RT);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-    const int t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices;
-    int adapter;
-    const int count = find_tile<TM>(p, t, tl, adapter);
-    if (count == 0 || adapter >= p.L) return;
-
-    const TX *xp[NT];
+    const int chunks = a.K / KC;                       // whole fragments; the last slice also takes what is left of K
+    const int c0 = (int)((long long)chunks * s / a.slices), c1 = (int)((long long)chunks * (s + 1) / a.slices);
+    const TX *xp[NB];
     const TW *mp[RT];
 #pragma unroll
-    for (int b = 0; b < NT; ++b) xp[b] = a.x + tl.rows[16 * b + j < count ? 16 * b + j : count - 1] * a.ldx + q * E;
+    for (int b = 0; b < NB; ++b) xp[b] = a.x + rows[16 * b + j < count ? 16 * b + j : count - 1] * a.ldx + q * E + (long long)(c0 + wave * UN) * KC;
 #pragma unroll
-    for (int b = 0; b < RT; ++b) mp[b] = a.m + adapter * a.sm + (16 * b + j < a.R ? 16 * b + j : a.R - 1) * a.ldm + q * E;
-    f32x4 acc[NT][RT];
+    for (int b = 0; b < RT; ++b) mp[b] = a.m + adapter * a.sm + (16 * b + j < a.R ? 16 * b + j : a.R - 1) * a.ldm + q * E + (long long)(c0 + wave * UN) * KC;
+    f32x4 acc[NB][RT];
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int c = 0; c < RT; ++c) acc[b][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    // this wave's whole fragments [c0, c1) of KC elements; the wave with the last ones also takes what is left of K
-    const int chunks = a.K / KC;
-    const int share = 4 * s + wave, shares = 4 * a.slices;
-    const int c0 = (int)((long long)chunks * share / shares), c1 = (int)((long long)chunks * (share + 1) / shares);
-    VX xa[UN][NT], xb[UN][NT];
+    VX xa[UN][NB], xb[UN][NB];
     VM ma[UN][RT], mb[UN][RT];
-    auto load = [&](VX(&xv)[UN][NT], VM(&mv)[UN][RT], int c) {
-        const long long k = (long long)c * KC;
+    auto walk = [&](int n) {                           // the pointers walk along: no address arithmetic but their steps
+#pragma unroll
+        for (int b = 0; b < NB; ++b) xp[b] += n * KC;
+#pragma unroll
+        for (int b = 0; b < RT; ++b) mp[b] += n * KC;
+    };
+    auto load = [&](VX(&xv)[UN][NB], VM(&mv)[UN][RT]) {
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
 #pragma unroll
-            for (int b = 0; b < NT; ++b) xv[u][b] = F::load(xp[b] + k + u * KC);
+            for (int b = 0; b < NB; ++b) xv[u][b] = load_lane<VX>(xp[b] + u * KC, E);
 #pragma unroll
-            for (int b = 0; b < RT; ++b) mv[u][b] = F::load(mp[b] + k + u * KC);
+            for (int b = 0; b < RT; ++b) mv[u][b] = load_lane<VM>(mp[b] + u * KC, E);
         }
+        walk(4 * UN);
     };
-    auto multiply = [&](const VX(&xv)[UN][NT], const VM(&mv)[UN][RT]) {
+    auto multiply1 = [&](const VX(&xv)[NB], const VM(&mv)[RT]) {     // neighbouring instructions on different accumulators
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
+        for (int e = 0; e < F::STEPS; ++e)
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) acc[b][r] = F::mma(xv[u][b], mv[u][r], acc[b][r]);
+                for (int r = 0; r < RT; ++r) acc[b][r] = F::mma(xv[b], mv[r], e, acc[b][r]);
     };
-    int c = c0;
-    if (c + UN <= c1) {
-        load(xa, ma, c);
-        c += UN;
-        for (;;) {
-            if (c + UN > c1) {
-                multiply(xa, ma);
-                break;
-            }
-            load(xb, mb, c);
-            c += UN;
+    auto multiply = [&](const VX(&xv)[UN][NB], const VM(&mv)[UN][RT]) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) multiply1(xv[u], mv[u]);
+    };
+    const int groups = (c1 - c0) / (4 * UN);
+    if (groups > 0) {
+        load(xa, ma);
+        for (int g = 1;; g += 2) {
+            if (g < groups) load(xb, mb);
             multiply(xa, ma);
-            if (c + UN > c1) {
-                multiply(xb, mb);
-                break;
-            }
-            load(xa, ma, c);
-            c += UN;
+            if (g >= groups) break;
+            if (g + 1 < groups) load(xa, ma);
             multiply(xb, mb);
+            if (g + 1 >= groups) break;
         }
     }
-    for (; c < c1; ++c) {
-        const long long k = (long long)c * KC;
-        VX xv[NT];
+    // single fragments behind the last whole group in turn, then what is left of K: zeros on both sides behind the end
+    const int rest = c0 + groups * 4 * UN, end = c1 + (s == a.slices - 1 && chunks * KC < a.K ? 1 : 0);
+    walk(wave - wave * UN);
+    for (int c = rest + wave; c < end; c += 4) {
+        const int left = c < c1 ? E : a.K - c * KC - q * E;
+        VX xv[NB];
         VM mv[RT];
 #pragma unroll
-        for (int b = 0; b < NT; ++b) xv[b] = F::load(xp[b] + k);
+        for (int b = 0; b < NB; ++b) xv[b] = load_lane<VX>(xp[b], left);
 #pragma unroll
-        for (int b = 0; b < RT; ++b) mv[b] = F::load(mp[b] + k);
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[b][r] = F::mma(xv[b], mv[r], acc[b][r]);
+        for (int b = 0; b < RT; ++b) mv[b] = load_lane<VM>(mp[b], left);
+        multiply1(xv, mv);
+        walk(4);
     }
-    if (share == shares - 1 && chunks * KC < a.K) {     // zeros on both sides behind the end: nothing there takes part
-        const int k = chunks * KC, left = a.K - k - q * E;
-        VX xv[NT];
-        VM mv[RT];
+    join_waves<NB, NT, RT>(acc, red);
+}
+
+// The staged form.  One operand's rows of a stage: which pieces this thread carries, and where they go.
+template <class T, int ROWS, int KS>
+struct Carrier {
+    static constexpr int E = 16 / sizeof(T), PPR = KS / E, LOADS = ROWS * PPR / 256, STEP = 256 / PPR;
+    static_assert(ROWS * PPR % 256 == 0 && PPR <= 256 && 256 % PPR == 0, "a stage is whole loads");
+    const T *src[LOADS];
+    u32x4 reg[LOADS];
+    // row(i) -> pointer to the row's first element of this slice
+    template <class F>
+    __device__ void start(const F &row) {
+        const int piece = threadIdx.x % PPR, first = threadIdx.x / PPR;
 #pragma unroll
-        for (int b = 0; b < NT; ++b) xv[b] = load_tail<VX>(xp[b] + k, E, left);
-#pragma unroll
-        for (int b = 0; b < RT; ++b) mv[b] = load_tail<VM>(mp[b] + k, E, left);
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) acc[b][r] = F::mma(xv[b], mv[r], acc[b][r]);
+        for (int i = 0; i < LOADS; ++i) src[i] = row(first + i * STEP) + piece * E;
     }
+    __device__ void load(int left) {                                   // left: elements of the slice from the stage on
+        const int mine = left - (int)(threadIdx.x % PPR) * E;
+        if (left >= KS) {
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+            for (int i = 0; i < LOADS; ++i) reg[i] = ((const Piece_m *)src[i])->v;
+        } else {
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+            for (int i = 0; i < LOADS; ++i) reg[i] = load_piece(src[i], mine);
+        }
 #pragma unroll
-            for (int v = 0; v < 4; ++v) red[wave][(16 * b + 4 * q + v) * R16 + 16 * r + j] = acc[b][r][v];
-    __syncthreads();
-    float *part = a.part + (long long)s * p.N * a.R;
-    for (int e = tid; e < count * R16; e += 256) {
-        const int row = e / R16, r = e % R16;
-        if (r < a.R) part[(long long)tl.rows[row] * a.R + r] = red[0][e] + red[1][e] + red[2][e] + red[3][e];
+        for (int i = 0; i < LOADS; ++i) src[i] += KS;
     }
+    __device__ void store(u32x4 *lds) const {
+        const int piece = threadIdx.x % PPR, first = threadIdx.x / PPR;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) lds[(first + i * STEP) * PPR + (piece ^ ((first + i * STEP) & (PPR < 16 ? PPR - 1 : 15)))] = reg[i];
+    }
+};
+
+template <class T, int KS>
+__device__ inline u32x4 fragment(const u32x4 *lds, int row, int piece) {
+    constexpr int PPR = KS * sizeof(T) / 16;
+    return lds[row * PPR + (piece ^ (row & (PPR < 16 ? PPR - 1 : 15)))];
+}
+
+template <class TX, class TW, int NB, int NT, int RT>
+__device__ inline void contract_staged(const ContractArgs<TX, TW> &a, const int *rows, int count, int adapter, int s, u32x4 *lds) {
+    constexpr int R16 = 16 * RT, KS = stage_elements(NT, RT, sizeof(TX), sizeof(TW)), E = 16 / sizeof(TX), KC = 4 * E;
+    constexpr int FRAGMENTS = KS / KC / 4;             // of a stage, for each wave
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
+    const int chunks = (a.K + KC - 1) / KC;            // slices are cut between fragments
+    const int k0 = (int)((long long)chunks * s / a.slices) * KC, k9 = (int)((long long)chunks * (s + 1) / a.slices) * KC, k1 = k9 < a.K ? k9 : a.K;
+    u32x4 *lx = lds, *lm = lds + 16 * NB * (KS * sizeof(TX) / 16);
+    Carrier<TX, 16 * NB, KS> cx;
+    Carrier<TW, R16, KS> cm;
+    cx.start([&](int i) { return a.x + rows[i < count ? i : count - 1] * a.ldx + k0; });
+    cm.start([&](int i) { return a.m + adapter * a.sm + (i < a.R ? i : a.R - 1) * a.ldm + k0; });
+    f32x4 acc[NB][RT];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < RT; ++c) acc[b][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int k = k0;
+    cx.load(k1 - k);
+    cm.load(k1 - k);
+    for (;;) {
+        cx.store(lx);
+        cm.store(lm);
+        __syncthreads();
+        k += KS;
+        if (k < k1) {
+            cx.load(k1 - k);
+            cm.load(k1 - k);
+        }
+#pragma unroll
+        for (int f = 0; f < FRAGMENTS; ++f) {
+            const int g = f * 4 + wave;
+            if constexpr (sizeof(TX) == 2) {
+                bf16x8 xv[NB], mv[RT];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) xv[b] = __builtin_bit_cast(bf16x8, fragment<TX, KS>(lx, 16 * b + j, 4 * g + q));
+#pragma unroll
+                for (int r = 0; r < RT; ++r) mv[r] = __builtin_bit_cast(bf16x8, fragment<TW, KS>(lm, 16 * r + j, 4 * g + q));
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[b], mv[r], acc[b][r], 0, 0, 0);
+            } else {                                   // lane (j, q) has k = 4 q .. 4 q + 3: four steps with k in another order
+                f32x4 xv[NB], mv[RT];
+#pragma unroll
+                for (int b = 0; b < NB; ++b) xv[b] = __builtin_bit_cast(f32x4, fragment<TX, KS>(lx, 16 * b + j, 4 * g + q));
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    if constexpr (sizeof(TW) == 4) {
+                        mv[r] = __builtin_bit_cast(f32x4, fragment<TW, KS>(lm, 16 * r + j, 4 * g + q));
+                    } else {                           // float32 gradients against bf16 weights: widened, exact
+                        const bf16x8 w = __builtin_bit_cast(bf16x8, fragment<TW, KS>(lm, 16 * r + j, 2 * g + (q >> 1)));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mv[r][e] = (float)(q & 1 ? w[4 + e] : w[e]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[b][e], mv[r][e], acc[b][r], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+        if (k >= k1) break;
+    }
+    join_waves<NB, NT, RT>(acc, (float *)lds);
+}
+
+template <class TX, class TW, int NT, int RT, bool STAGED>
+__global__ __launch_bounds__(256, 2) void contract_kernel(const ContractArgs<TX, TW> a, const Plan p) {
+    constexpr int TM = 16 * NT, R16 = 16 * RT, KS = stage_elements(NT, RT, sizeof(TX), sizeof(TW));
+    constexpr int STAGE = STAGED ? (TM * sizeof(TX) + R16 * sizeof(TW)) * KS : 0, SUMS = 2 * TM * R16 * 4, BYTES = STAGE > SUMS ? STAGE : SUMS;
+    __shared__ TileLds tl;
+    __shared__ u32x4 lds[BYTES / 16];
+    float *red = (float *)lds;
+    const int tid = threadIdx.x;
+    const int t = blockIdx.x / a.slices, s = blockIdx.x - t * a.slices;
+    int adapter;
+    const int count = __builtin_amdgcn_readfirstlane(find_tile(p, t, TM, tl, adapter));
+    if (count == 0 || adapter >= p.L) return;
+    auto tile = [&](auto nb) {
+        constexpr int NB = decltype(nb)::value;
+        if constexpr (STAGED) contract_staged<TX, TW, NB, NT, RT>(a, tl.rows, count, adapter, s, lds);
+        else contract_direct<TX, TW, NB, NT, RT>(a, tl.rows, count, adapter, s, red);
+    };
+    if (NT == 1 || count <= 16) tile(std::integral_constant<int, 1>());
+    else if (NT == 2 || count <= 32) tile(std::integral_constant<int, 2>());
+    else if (count <= 48) tile(std::integral_constant<int, NT == 4 ? 3 : 2>());
+    else tile(std::integral_constant<int, NT>());
+    float *part = a.part + (long long)s * p.N * R16;
+    for (int e = 4 * tid; e < count * R16; e += 1024)
+        *(f32x4 *)(part + (long long)tl.rows[e / R16] * R16 + e % R16) = *(const f32x4 *)(red + e) + *(const f32x4 *)(red + TM * R16 + e);
 }
 
 // --------------------------------------------------------------------------------------------------------------- expand
@@ -349,33 +525,50 @@ __device__ inline f32x4 load4(const T *p, int left) {
     return v;
 }
 
-// dst[row][r] (row stride ld) = f * sum_s part[s][rows[row]][r], zero for r in [R, R16); also stored to keep, without f
+// dst[row][r] (row stride LD) = f * sum_s part[s][rows[row]][r]; also stored to keep (N, R), without f.  A row of part has ldp
+// values: R16 (a kernel's partial sums; repeats for r in [R, R16), taken as zeros) or R (the caller's h).
+__device__ inline void put4(float *dst, f32x4 v, float f, float *keep, long long n, int r, int R) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const bool live = r + e < R;
+        dst[e] = live ? f * v[e] : 0.f;
+        if (keep && live) keep[n * R + r + e] = v[e];
+    }
+}
 template <int R16, int LD>
-__device__ inline void join(float *dst, float *lds, const float *__restrict__ part, int slices, long long slab, const int *rows, int count,
-                            int batch, int R, float f, float *keep) {
+__device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ part, int ldp, int slices, int N, const int *rows, int count, int R,
+                            float f, float *keep) {
+    constexpr int R4 = R16 / 4;
     const int tid = threadIdx.x;
-    if (batch * R16 <= 128 && slices > 4) {           // a small batch: several threads to a value, as many for every tile
-        const int n = batch * R16, groups = 256 / n;
-        const int e = tid % n, g = tid / n, row = e / R16, r = e % R16;
-        float v = 0.f;
-        if (g < groups && row < count && r < R)
-            for (int s = g; s < slices; s += groups) v += part[s * slab + (long long)rows[row] * R + r];
-        lds[tid] = v;
-        __syncthreads();
-        if (row < count && tid < n) {
-            float sum = 0.f;
-            for (int k = 0; k < groups; ++k) sum += lds[k * n + tid];
-            dst[row * LD + r] = f * sum;
-            if (keep && r < R) keep[(long long)rows[row] * R + r] = sum;
-        }
-    } else {
+    const long long slab = (long long)N * ldp;
+    if (ldp != R16) {
         for (int e = tid; e < count * R16; e += 256) {
             const int row = e / R16, r = e % R16;
-            float v = 0.f;
-            if (r < R)
-                for (int s = 0; s < slices; ++s) v += part[s * slab + (long long)rows[row] * R + r];
-            dst[row * LD + r] = f * v;
-            if (keep && r < R) keep[(long long)rows[row] * R + r] = v;
+            dst[row * LD + r] = r < R ? f * part[(long long)rows[row] * ldp + r] : 0.f;
+        }
+    } else if (N * R4 <= 64 && slices > 4) {          // a small batch: several threads to a value, as many for every tile
+        const int n = N * R4, groups = 256 / n, e = tid % n, g = tid / n, row = e / R4, r = 4 * (e % R4);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (g < groups && row < count) {
+            const float *src = part + (long long)rows[row] * ldp + r;
+#pragma unroll 4
+            for (int s = g; s < slices; s += groups) v += *(const f32x4_m *)(src + s * slab);
+        }
+        lds[tid] = v;
+        __syncthreads();
+        if (tid < n && row < count) {
+            f32x4 sum = v;
+            for (int k = 1; k < groups; ++k) sum += lds[k * n + tid];
+            put4(dst + row * LD + r, sum, f, keep, rows[row], r, R);
+        }
+    } else {
+        for (int e = tid; e < count * R4; e += 256) {
+            const int row = e / R4, r = 4 * (e % R4);
+            const float *src = part + (long long)rows[row] * ldp + r;
+            f32x4 v = *(const f32x4_m *)src;
+#pragma unroll 8
+            for (int s = 1; s < slices; ++s) v += *(const f32x4_m *)(src + s * slab);
+            put4(dst + row * LD + r, v, f, keep, rows[row], r, R);
         }
     }
     __syncthreads();
@@ -383,12 +576,13 @@ __device__ inline void join(float *dst, float *lds, const float *__restrict__ pa
 
 template <class T>
 struct ExpandArgs {
-    const float *part;         // (slices, N, R)
+    const float *part;         // (slices, N, R16)
     const T *m;                // (L, R, U) strides sm, ldm
     const float *scale;        // (L)
     float *out, *keep;         // (N, U) stride ldo; (N, R) or null
     long long ldm, sm, ldo;
-    int U, R, slices, blocks, accumulate;
+    int U, R, slices, spans, span, accumulate;     // a workgroup takes `span` blocks of 256 columns; `spans` of them cover U
+    int TM, subs;              // rows of a tile; a workgroup takes 16 NT of them, `subs` workgroups cover the tile
 };
 
 template <class T, int NT, int RT>
@@ -396,62 +590,72 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
     constexpr int TM = 16 * NT, R16 = 16 * RT, LD = R16 + 4, STEPS = R16 / 4;
     __shared__ TileLds tl;
     __shared__ __attribute__((aligned(16))) float h[TM * LD];
-    __shared__ float sums[256];
+    __shared__ f32x4 sums[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-    const int t = blockIdx.x / a.blocks, block = blockIdx.x - t * a.blocks;
+    const int whole = blockIdx.x / a.spans, first = (blockIdx.x - whole * a.spans) * a.span, t = whole / a.subs, sub = whole - t * a.subs;
     int adapter;
-    const int count = find_tile<TM>(p, t, tl, adapter);
-    if (count == 0) return;
-    float *keep = block == 0 ? a.keep : nullptr;
-    const int u = block * 256 + wave * 64 + 4 * j, left = a.U - u;
+    const int all = find_tile(p, t, a.TM, tl, adapter) - sub * TM, count = all < TM ? all : TM;
+    if (count <= 0) return;
+    const int *rows = tl.rows + sub * TM;
+    float *keep = first == 0 ? a.keep : nullptr;
+    const int u_end = (first + a.span) * 256 < a.U ? (first + a.span) * 256 : a.U;
     if (adapter >= p.L) {                              // no adapter: zeros (or out as it is); an index behind the bank: NaN
         for (int row = 0; row < count; ++row) {
-            const int n = tl.rows[row];
+            const int n = rows[row];
             const bool bad = p.index[n] >= 0;
             const float v = bad ? __builtin_nanf("") : 0.f;
-            const int c = block * 256 + tid;
-            if (c < a.U && (bad || !a.accumulate)) a.out[n * a.ldo + c] = v;
+            if (bad || !a.accumulate)
+                for (int c = first * 256 + tid; c < u_end; c += 256) a.out[n * a.ldo + c] = v;
             if (keep && tid < a.R) keep[(long long)n * a.R + tid] = v;
         }
         return;
     }
     f32x4 m[STEPS];                                    // step k of lane (j, q): rank q * STEPS + k, the same order as h's
-    const T *mp = a.m + adapter * a.sm + u;
+    int u = first * 256 + wave * 64 + 4 * j;
+    const T *mp = a.m + adapter * a.sm;
+    auto load = [&]() {
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k) {
-        const int r = q * STEPS + k;
-        m[k] = r < a.R && left > 0 ? load4(mp + r * a.ldm, left) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
-    join<R16, LD>(h, sums, a.part, a.slices, (long long)p.N * a.R, tl.rows, count, p.N, a.R, a.scale[adapter], keep);
-    if (block * 256 + wave * 64 >= a.U) return;
-#pragma unroll
-    for (int b = 0; b < NT; ++b) {
-        if (16 * b >= count) break;
-        f32x4 acc[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < STEPS; k += 4) {
-            const f32x4 hv = *(const f32x4 *)(h + (16 * b + j) * LD + q * STEPS + k);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[e], m[k + e][c], acc[c], 0, 0, 0);
+        for (int k = 0; k < STEPS; ++k) {
+            const int r = q * STEPS + k;
+            m[k] = r < a.R && u < a.U ? load4(mp + r * a.ldm + u, a.U - u) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
+    };
+    load();
+    for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
+    join<R16, LD>(h, sums, a.part, R16, a.slices, p.N, rows, count, a.R, a.scale[adapter], keep);
+    for (;;) {
+        const int left = a.U - u;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int row = 16 * b + 4 * q + v;
-            if (row >= count || left <= 0) continue;
-            float *o = a.out + tl.rows[row] * a.ldo + u;
-            f32x4 val = {acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
-            if (left >= 4) {
-                if (a.accumulate) val += load4(o);
-                *(f32x4_m *)o = val;
-            } else {
-                for (int e = 0; e < left; ++e) o[e] = a.accumulate ? o[e] + val[e] : val[e];
+        for (int b = 0; b < NT; ++b) {
+            if (16 * b >= count) break;
+            f32x4 acc[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < STEPS; k += 4) {
+                const f32x4 hv = *(const f32x4 *)(h + (16 * b + j) * LD + q * STEPS + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[e], m[k + e][c], acc[c], 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int row = 16 * b + 4 * q + v;
+                if (row >= count || left <= 0) continue;
+                float *o = a.out + rows[row] * a.ldo + u;
+                f32x4 val = {acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
+                if (left >= 4) {
+                    if (a.accumulate) val += load4(o);
+                    *(f32x4_m *)o = val;
+                } else {
+                    for (int e = 0; e < left; ++e) o[e] = a.accumulate ? o[e] + val[e] : val[e];
+                }
             }
         }
+        u += 256;
+        if (u - 4 * j >= u_end) break;
+        load();
     }
 }
 
@@ -462,11 +666,11 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
 // and take a quarter of the rows each (few adapters: four times the workgroups).
 template <class T>
 struct RowsArgs {
-    const float *part;         // (slices, N, R)
+    const float *part;         // (slices, N, ldp)
     const T *x;                // (N, K) stride ldx
     float *out;                // (L, R, K) strides so, ldo
     long long ldx, ldo, so;
-    int K, slices, blocks;
+    int K, slices, ldp, blocks;
 };
 
 struct RowsLds {
@@ -513,15 +717,21 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
             tl.rows[place - r0] = tid;
         }
         __syncthreads();
-        for (int e = tid; e < (padded - count) * LD; e += 256) g[count * LD + e] = 0.f;
-        join<R16, LD>(g, red, a.part, a.slices, (long long)p.N * R, tl.rows, count, p.N, R, f, nullptr);
-        for (int s0 = SPLIT ? 16 * wave : 0; s0 < count; s0 += SPLIT ? 64 : 16) {
-            f32x4 x[4];
+        f32x4 x[4], ahead[4];                          // in flight while h is joined and while the rows before multiply
+        auto load = [&](f32x4(&v)[4], int s0) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const int row = s0 + 4 * s + q;
-                x[s] = row < count && left > 0 ? load4(a.x + tl.rows[row] * a.ldx + k, left) : f32x4{0.f, 0.f, 0.f, 0.f};
+                v[s] = row < count && left > 0 ? load4(a.x + tl.rows[row] * a.ldx + k, left) : f32x4{0.f, 0.f, 0.f, 0.f};
             }
+        };
+        const int stride = SPLIT ? 64 : 16;
+        int s0 = SPLIT ? 16 * wave : 0;
+        load(x, s0);
+        for (int e = tid; e < (padded - count) * LD; e += 256) g[count * LD + e] = 0.f;
+        join<R16, LD>(g, (f32x4 *)red, a.part, a.ldp, a.slices, p.N, tl.rows, count, R, f, nullptr);
+        for (; s0 < count; s0 += stride) {
+            if (!SPLIT) load(ahead, s0 + stride);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -530,6 +740,9 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
 #pragma unroll
                     for (int c = 0; c < 4; ++c) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(gv, x[s][c], acc[t][c], 0, 0, 0);
                 }
+            if (!SPLIT)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) x[s] = ahead[s];
         }
     }
     float *out = a.out + i * a.so;
@@ -572,7 +785,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs<T> a, const Ro
     constexpr int R16 = 16 * RT, LD = RT == 1 ? 16 : R16 + 16;
     __shared__ RowsLds tl;
     __shared__ __attribute__((aligned(16))) float g[64 * LD];
-    __shared__ __attribute__((aligned(16))) float red[SPLIT ? 4096 : 256];
+    __shared__ __attribute__((aligned(16))) float red[SPLIT ? 4096 : 1024];
     if ((int)blockIdx.x < a_blocks) rows_tile<T, RT, SPLIT>(a, p, scale, R, blockIdx.x, g, red, tl);
     else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x - a_blocks, g, red, tl);
 }
@@ -622,8 +835,8 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     y.offs = take(y.sorted ? 4 * ((size_t)L + 1) : 0);
     y.tiles = take(y.sorted ? 16 * (size_t)y.max_tiles : 0);
     y.ntiles = take(y.sorted ? 4 : 0);
-    y.part = take(4 * (size_t)y.slices * N * R);
-    y.part2 = take(4 * (size_t)y.slices2 * N * R);
+    y.part = take(64 * (size_t)y.slices * N * y.rt);
+    y.part2 = take(64 * (size_t)y.slices2 * N * y.rt);
     y.bytes = at < 256 ? 256 : at;
     return y;
 }
@@ -660,7 +873,14 @@ void contract(const Layout &y, const Plan &p, const TX *x, long long ldx, const 
               int slices, hipStream_t s) {
     const ContractArgs<TX, TM> a = {x, m, part, ldx, ldm, sm, K, R, slices};
     const dim3 grid((unsigned)(y.max_tiles * slices));
-#define CALL(NT, RT) contract_kernel<TX, TM, NT, RT><<<grid, dim3(256), 0, s>>>(a, p)
+    // staged where tall tiles fill the chip with long slices: 4096 rows x 12544 of rank 64 take 104 us against 115 to 130 direct;
+    // direct where latency counts: one row 4.7 us against 5.5, 2048 rows x 1470 of rank 32 13.0 against 15.9
+    const bool staged = y.nt > 1 && y.max_tiles * slices >= 512 && K / slices * (int)sizeof(TX) >= 2048;
+#define CALL(NT, RT)                                                                                 \
+    do {                                                                                             \
+        if (NT > 1 && staged) contract_kernel<TX, TM, NT, RT, (NT > 1)><<<grid, dim3(256), 0, s>>>(a, p); \
+        else contract_kernel<TX, TM, NT, RT, false><<<grid, dim3(256), 0, s>>>(a, p);                \
+    } while (0)
     TY1_BY_TILE(y, CALL);
 #undef CALL
 }
@@ -668,11 +888,18 @@ void contract(const Layout &y, const Plan &p, const TX *x, long long ldx, const 
 template <class T>
 void expand(const Layout &y, const Plan &p, const float *part, int slices, const T *m, long long ldm, long long sm, const float *scale, float *out,
             long long ldo, float *keep, int U, int R, int accumulate, hipStream_t s) {
-    const int blocks = (U + 255) / 256;
-    const ExpandArgs<T> a = {part, m, scale, out, keep, ldm, sm, ldo, U, R, slices, blocks, accumulate};
-    const dim3 grid((unsigned)(y.max_tiles * blocks));
+    // Few workgroups: 16 rows each instead of the tile's height (4096 rows x 539 of rank 64: 29 us with 64 rows a workgroup).
+    // Plenty: several blocks of columns each, h is joined once for all of them.
+    const int blocks = (U + 255) / 256, nt = (long long)y.max_tiles * blocks < 1024 ? 1 : y.nt, subs = y.nt / nt;
+    int span = (int)((long long)y.max_tiles * blocks / 1024);
+    span = span < 1 ? 1 : span > blocks ? blocks : span;
+    const int spans = (blocks + span - 1) / span;
+    const ExpandArgs<T> a = {part, m, scale, out, keep, ldm, sm, ldo, U, R, slices, spans, span, accumulate, 16 * y.nt, subs};
+    const dim3 grid((unsigned)(y.max_tiles * subs * spans));
+    Layout z = y;
+    z.nt = nt;
 #define CALL(NT, RT) expand_kernel<T, NT, RT><<<grid, dim3(256), 0, s>>>(a, p)
-    TY1_BY_TILE(y, CALL);
+    TY1_BY_TILE(z, CALL);
 #undef CALL
 }
 
@@ -702,7 +929,7 @@ int forward(const char *what, const T *x, const T *a, const T *b, const int32_t 
     const Layout y = layout(N, K, U, L, R, false);
     TY1_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y.bytes, "%s: workspace null, not 16-byte aligned, or %zu bytes where %zu are needed", what,
                 ws_bytes, y.bytes);
-    if (check_grid(what, y, y.slices) || check_grid(what, y, (U + 255ll) / 256)) return 1;
+    if (check_grid(what, y, y.slices) || check_grid(what, y, 4 * ((U + 255ll) / 256))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_forward", s, 2.0 * N * R * ((double)K + U), sizeof(T) * ((double)N * K + (double)(L < N ? L : N) * R * ((double)K + U)) + 4.0 * N * U);
     const Plan p = make_plan(y, (char *)ws, index, N, L, s);
@@ -727,10 +954,10 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     TY1_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y.bytes, "%s: workspace null, not 16-byte aligned, or %zu bytes where %zu are needed", what,
                 ws_bytes, y.bytes);
     // few adapters: 64 columns a workgroup and the rows split over its waves; enough of them: 256 columns, whole waves
-    const bool split = (long long)L * ((K + 255) / 256 + (U + 255) / 256) < 1024;
+    const bool split = (long long)L * ((K + 255) / 256 + (U + 255) / 256) < 256;
     const long long ka = split ? (K + 63ll) / 64 : (K + 255ll) / 256, ub = split ? (U + 63ll) / 64 : (U + 255ll) / 256;
     TY1_REQUIRE(L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
-    if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, (K + 255ll) / 256))) return 1;
+    if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 4 * ((K + 255ll) / 256)))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_backward", s, 2.0 * N * R * (K * (dx ? 2.0 : 1.0) + 2.0 * U),
                         sizeof(T) * (double)N * K + 4.0 * N * U + 4.0 * L * R * ((double)K + U) + (dx ? 4.0 * N * K : 0.0));
@@ -741,8 +968,8 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
         contract(y, p, dz, lddz, b, ldb, sb, part, U, R, y.slices, s);
         if (!h) contract(y, p, x, ldx, a, lda, sa, part2, K, R, y.slices2, s);
     }
-    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, (int)ka};
-    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, h ? 1 : y.slices2, (int)ub};
+    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, 16 * y.rt, (int)ka};
+    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, h ? 1 : y.slices2, h ? R : 16 * y.rt, (int)ub};
     const dim3 grid((unsigned)(L * (ka + ub)));
 #define CALL(RT)                                                                                                                    \
     do {                                                                                                                            \

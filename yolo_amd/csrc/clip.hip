@@ -40,25 +40,124 @@ __device__ inline double block_sum(double v, double *lds) {
     return sum;
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_m __attribute__((ext_vector_type(4), aligned(4)));         // as it lies in memory: views of a bucket start anywhere
+typedef __bf16 bf16x4_m __attribute__((ext_vector_type(4), aligned(2)));
+
 // calls f(t, lo, hi) for every tensor that has values in this workgroup's share of the concatenation
 template <class F>
 __device__ inline void my_share(const Lists &ls, const F &f) {
-    const long long total = ls.start[ls.n], per = (total + gridDim.x - 1) / gridDim.x;
+    const long long total = ls.start[ls.n], per = (total + gridDim.x * 16ll - 1) / (gridDim.x * 16ll) * 16;
     const long long lo = per * blockIdx.x, hi = lo + per < total ? lo + per : total;
-    for (int t = 0; t < ls.n; ++t) {
+    if (lo >= hi) return;
+    int t = 0;
+    for (int step = kTensors / 2; step > 0; step >>= 1)
+        if (t + step < ls.n && ls.start[t + step] <= lo) t += step;
+    for (; t < ls.n && ls.start[t] < hi; ++t) {
         const long long a = lo > ls.start[t] ? lo : ls.start[t], b = hi < ls.start[t + 1] ? hi : ls.start[t + 1];
-        if (a < b) f(t, a - ls.start[t], b - ls.start[t]);
+        f(t, a - ls.start[t], b - ls.start[t]);
     }
+}
+
+// calls four(j) for groups of four values from lo on, UN of them a thread before the next (their loads in flight together), and
+// one(j) for the last values
+template <int UN, class Four, class One>
+__device__ inline void by_fours(long long lo, long long hi, const Four &four, const One &one) {
+    constexpr int W = 4 * kThreads;
+    const long long whole = lo + ((hi - lo) & ~3ll);
+    long long j = lo + 4 * threadIdx.x;
+    for (; j + (UN - 1) * W < whole; j += UN * W) {
+        typename Four::Values v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) v[u] = four.load(j + u * W);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) four.use(j + u * W, v[u]);
+    }
+    for (; j < whole; j += W) four.use(j, four.load(j));
+    if (whole + threadIdx.x < hi) one(whole + threadIdx.x);
+}
+
+__device__ inline f32x4 load4(const float *p) { return *(const f32x4_m *)p; }
+__device__ inline f32x4 load4(const bf16 *p) {
+    const bf16x4_m v = *(const bf16x4_m *)p;
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ inline void store4(float *p, f32x4 v) { *(f32x4_m *)p = v; }
+__device__ inline void store4(bf16 *p, f32x4 v) { *(bf16x4_m *)p = bf16x4_m{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]}; }
+__device__ inline float scaled(float g, double c) { return (float)((double)g * c); }
+
+template <class T>
+struct Square {
+    typedef f32x4 Values;
+    const T *g;
+    double *sum;
+    __device__ Values load(long long j) const { return load4(g + j); }
+    __device__ void use(long long, const Values &v) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *sum += (double)v[e] * (double)v[e];
+    }
+};
+
+template <class T>
+struct Scale {
+    typedef f32x4 Values;
+    const T *g;
+    T *out;
+    double c;
+    __device__ Values load(long long j) const { return load4(g + j); }
+    __device__ void use(long long j, Values v) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = scaled(v[e], c);
+        store4(out + j, v);
+    }
+};
+
+struct Adam {
+    struct Values {
+        f32x4 p, g, m, v;
+    };
+    float *p, *m, *v;
+    const float *g;
+    double c;
+    float rate, b1, b2, c1, c2, eps;
+    __device__ Values load(long long j) const { return {load4(p + j), load4(g + j), load4(m + j), load4(v + j)}; }
+    __device__ void step(float &pj, float gj, float &mj, float &vj) const {
+        gj = scaled(gj, c);
+        mj = b1 * mj + c1 * gj;
+        vj = b2 * vj + c2 * (gj * gj);
+        pj -= rate * mj / (sqrtf(vj) + eps);
+    }
+    __device__ void use(long long j, Values x) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float pe = x.p[e], me = x.m[e], ve = x.v[e];
+            step(pe, x.g[e], me, ve);
+            x.p[e] = pe;
+            x.m[e] = me;
+            x.v[e] = ve;
+        }
+        store4(p + j, x.p);
+        store4(m + j, x.m);
+        store4(v + j, x.v);
+    }
+};
+
+template <class T>
+__device__ inline void square_share(const T *g, long long lo, long long hi, double &sum) {
+    by_fours<4>(lo, hi, Square<T>{g, &sum}, [&](long long j) { sum += (double)(float)g[j] * (double)(float)g[j]; });
+}
+
+template <class T>
+__device__ inline void scale_share(const T *g, T *out, double c, long long lo, long long hi) {
+    by_fours<4>(lo, hi, Scale<T>{g, out, c}, [&](long long j) { out[j] = (T)scaled((float)g[j], c); });
 }
 
 __global__ __launch_bounds__(kThreads) void norm_kernel(const Lists ls, double *__restrict__ part) {
     __shared__ double lds[4];
     double sum = 0.0;
     my_share(ls, [&](int t, long long lo, long long hi) {
-        for (long long j = lo + threadIdx.x; j < hi; j += kThreads) {
-            const double v = ls.half >> t & 1 ? (double)(float)((const bf16 *)ls.a[t])[j] : (double)((const float *)ls.a[t])[j];
-            sum += v * v;
-        }
+        if (ls.half >> t & 1) square_share((const bf16 *)ls.a[t], lo, hi, sum);
+        else square_share((const float *)ls.a[t], lo, hi, sum);
     });
     sum = block_sum(sum, lds);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -84,26 +183,20 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(const Lists ls, const do
     __shared__ double lds[4];
     const double c = coefficient(part, parts, max_norm, norm, lds);
     my_share(ls, [&](int t, long long lo, long long hi) {
-        for (long long j = lo + threadIdx.x; j < hi; j += kThreads)
-            if (ls.half >> t & 1) ((bf16 *)ls.b[t])[j] = (bf16)(float)((double)(float)((const bf16 *)ls.a[t])[j] * c);
-            else ((float *)ls.b[t])[j] = (float)((double)((const float *)ls.a[t])[j] * c);
+        if (c == 1.0 && ls.a[t] == ls.b[t]) return;                    // in place and within the norm: the values are the result
+        if (ls.half >> t & 1) scale_share((const bf16 *)ls.a[t], (bf16 *)ls.b[t], c, lo, hi);
+        else scale_share((const float *)ls.a[t], (float *)ls.b[t], c, lo, hi);
     });
 }
 
 __global__ __launch_bounds__(kThreads) void adam_clip_kernel(const Lists ls, const double *__restrict__ part, int parts,
-                                                             double max_norm, float *norm, float lr_t, float b1, float b2, float c1, float c2, float eps) {
+                                                             double max_norm, float *norm, float rate, float b1, float b2, float c1,
+                                                             float c2, float eps) {
     __shared__ double lds[4];
     const double c = coefficient(part, parts, max_norm, norm, lds);
     my_share(ls, [&](int t, long long lo, long long hi) {
-        float *p = (float *)ls.a[t], *m = (float *)ls.c[t], *v = (float *)ls.d[t];
-        const float *g = (const float *)ls.b[t];
-        for (long long j = lo + threadIdx.x; j < hi; j += kThreads) {
-            const float gj = (float)((double)g[j] * c);
-            const float mj = b1 * m[j] + c1 * gj, vj = b2 * v[j] + c2 * (gj * gj);
-            m[j] = mj;
-            v[j] = vj;
-            p[j] -= lr_t * mj / (sqrtf(vj) + eps);
-        }
+        const Adam f = {(float *)ls.a[t], (float *)ls.c[t], (float *)ls.d[t], (const float *)ls.b[t], c, rate, b1, b2, c1, c2, eps};
+        by_fours<1>(lo, hi, f, [&](long long j) { f.step(f.p[j], f.g[j], f.m[j], f.v[j]); });
     });
 }
 
