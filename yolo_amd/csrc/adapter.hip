@@ -37,8 +37,7 @@ struct Plan {
     int N, L;
     const int *perm;           // (N) rows, stably sorted by class        | null: N <= kSelfPlan
     const int *offs;           // (L + 1) first place of each class in perm
-    const int4 *tiles;         // {class, first place, rows, -}
-    const int *ntiles;
+    const int4 *tiles;         // {class, first place, rows, -}, the unused ones without rows
 };
 
 __device__ inline int class_of(int i, int L) { return i < 0 || i >= L ? L : i; }
@@ -108,8 +107,7 @@ __device__ inline int tile_by_ballots(const Plan &p, int t, int TM, TileLds &lds
 __device__ inline int find_tile(const Plan &p, int t, int TM, TileLds &lds, int &adapter) {
     const int tid = threadIdx.x;
     if (p.perm) {
-        if (t >= *p.ntiles) return 0;
-        const int4 tile = p.tiles[t];
+        const int4 tile = p.tiles[t];                  // (no rows: behind the last tile)
         if (tid < tile.z) lds.rows[tid] = p.perm[tile.y + tid];
         adapter = tile.x;
         __syncthreads();
@@ -126,16 +124,27 @@ __device__ inline int find_tile(const Plan &p, int t, int TM, TileLds &lds, int 
 // ranked by ballots over the bits of the class.
 __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ index, int N, int L, int waves, int bits, int TM,
                                                     int *__restrict__ perm, int *__restrict__ offs, int4 *__restrict__ tiles,
-                                                    int *__restrict__ ntiles) {
+                                                    int max_tiles) {
     extern __shared__ int hist[];                     // [waves][L + 1]
     __shared__ long long scan[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, C = L + 1;
     const int per = ((N + waves - 1) / waves + 63) & ~63;
     const long long lo = (long long)wave * per, hi = lo + per < N ? lo + per : N;
+    constexpr int KEEP = 8;                           // the first rows' classes stay in registers between the two passes
+    int kept[KEEP];
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const long long n = lo + 64 * k + lane;
+        kept[k] = wave < waves && n < hi ? class_of(index[n], L) : -1;
+    }
     for (int c = tid; c < waves * C; c += 1024) hist[c] = 0;
     __syncthreads();
-    if (wave < waves)
-        for (long long n = lo + lane; n < hi; n += 64) atomicAdd(&hist[wave * C + class_of(index[n], L)], 1);
+    if (wave < waves) {
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k)
+            if (kept[k] >= 0) atomicAdd(&hist[wave * C + kept[k]], 1);
+        for (long long n = lo + 64 * KEEP + lane; n < hi; n += 64) atomicAdd(&hist[wave * C + class_of(index[n], L)], 1);
+    }
     __syncthreads();
     long long carry = 0;                              // rows in the low half, tiles in the high half
     for (int c0 = 0; c0 < C; c0 += 1024) {
@@ -170,23 +179,28 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
         }
         __syncthreads();
     }
-    if (tid == 0) *ntiles = (int)(carry >> 32);
+    for (int t = (int)(carry >> 32) + tid; t < max_tiles; t += 1024) tiles[t] = make_int4(0, 0, 0, 0);
     if (wave < waves) {
         volatile int *mine = hist + wave * C;
-        for (long long n0 = lo; n0 < hi; n0 += 64) {
-            const long long n = n0 + lane;
-            const int cls = n < hi ? class_of(index[n], L) : -1;
-            unsigned long long same = __ballot(n < hi);
+        auto put = [&](int cls, long long n) {
+            unsigned long long same = __ballot(cls >= 0);
             for (int b = 0; b < bits; ++b) {
                 const unsigned long long set = __ballot(cls >> b & 1);
                 same &= cls >> b & 1 ? set : ~set;
             }
-            if (n < hi) {
+            if (cls >= 0) {
                 const int rank = __popcll(same & ((1ull << lane) - 1));
                 const int place = mine[cls];
                 if (rank == 0) mine[cls] = place + __popcll(same);
                 perm[place + rank] = (int)n;
             }
+        };
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k)
+            if (lo + 64 * k < hi) put(kept[k], lo + 64 * k + lane);
+        for (long long n0 = lo + 64 * KEEP; n0 < hi; n0 += 64) {
+            const long long n = n0 + lane;
+            put(n < hi ? class_of(index[n], L) : -1, n);
         }
     }
 }
@@ -613,18 +627,24 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
     f32x4 m[STEPS];                                    // step k of lane (j, q): rank q * STEPS + k, the same order as h's
     int u = first * 256 + wave * 64 + 4 * j;
     const T *mp = a.m + adapter * a.sm;
-    auto load = [&]() {
+    auto load = [&](f32x4 *v, int c) {
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
             const int r = q * STEPS + k;
-            m[k] = r < a.R && u < a.U ? load4(mp + r * a.ldm + u, a.U - u) : f32x4{0.f, 0.f, 0.f, 0.f};
+            v[k] = r < a.R && c < a.U ? load4(mp + r * a.ldm + c, a.U - c) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
     };
-    load();
+    load(m, u);
     for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
     join<R16, LD>(h, sums, a.part, R16, a.slices, p.N, rows, count, a.R, a.scale[adapter], keep);
+    float *at[NT][4];
+#pragma unroll
+    for (int b = 0; b < NT; ++b)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) at[b][v] = a.out + rows[16 * b + 4 * q + v < count ? 16 * b + 4 * q + v : 0] * a.ldo;
     for (;;) {
         const int left = a.U - u;
+        const bool more = u - 4 * j + 256 < u_end;
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             if (16 * b >= count) break;
@@ -641,9 +661,8 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
             }
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const int row = 16 * b + 4 * q + v;
-                if (row >= count || left <= 0) continue;
-                float *o = a.out + rows[row] * a.ldo + u;
+                if (16 * b + 4 * q + v >= count || left <= 0) continue;
+                float *o = at[b][v] + u;
                 f32x4 val = {acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
                 if (left >= 4) {
                     if (a.accumulate) val += load4(o);
@@ -653,141 +672,167 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
                 }
             }
         }
+        if (!more) break;
         u += 256;
-        if (u - 4 * j >= u_end) break;
-        load();
+        load(m, u);
     }
 }
 
 // ----------------------------------------------------------------------------------------------------------------- rows
-// out[i][r][k] = f sum over the rows n of adapter i of g[n][r] x[n][k], g = sum_s part[s]: one wave per 64 columns, lane (j, q)
-// holding four consecutive ones of row 4 step + q, so that loads of x and stores of out are 256 bytes a row.  Bound by reading
-// x and writing out once.  Two such products (A's gradient and B's) share a launch.  SPLIT: the four waves share the columns
-// and take a quarter of the rows each (few adapters: four times the workgroups).
+// out[i][r][k] = scale[i] sum over the rows n of adapter i of g[n][r] x[n][k], g = sum_s part[s]: lane (j, q) of a wave holds
+// four consecutive columns of row 4 step + q, so that loads of x and stores of out are 256 bytes a row.  Bound by reading x
+// and writing out once.  A wave runs through the adapter's rows by itself, 16 at a time, reading g from L2: a version that put
+// g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of rank 32: 81 us).  Two such products (A's
+// gradient and B's) share a launch.
+//   few rows to an adapter: a wave has 64 columns and all rows, a workgroup 256 columns;
+//   many (SPLIT): the four waves have the same 64 columns and a quarter of the rows each, joined in LDS (128 or 256 columns to
+//   a wave read g less often and measured slower, 54 against 61 and 99 us: the adapter with the most rows has too few waves).
 template <class T>
 struct RowsArgs {
     const float *part;         // (slices, N, ldp)
     const T *x;                // (N, K) stride ldx
     float *out;                // (L, R, K) strides so, ldo
     long long ldx, ldo, so;
-    int K, slices, ldp, blocks;
+    int K, slices, ldp, blocks, ranks;     // `blocks` workgroups to an adapter and 64 ranks, `ranks` times 64 ranks
 };
 
-struct RowsLds {
-    int rows[64];
-    int wave_rows[4];
-};
+// the rows of adapter i in ascending order, up to kSelfPlan of them: every wave writes and reads the same list
+template <int W>
+__device__ inline int rows_by_ballots(const Plan &p, int i, int *rows) {
+    const int lane = threadIdx.x & 63;
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int n = 64 * w + lane;
+        const bool mine = n < p.N && p.index[n] == i;
+        const unsigned long long vote = __ballot(mine);
+        if (mine) rows[total + __popcll(vote & ((1ull << lane) - 1))] = n;
+        total += __popcll(vote);
+    }
+    __builtin_amdgcn_wave_barrier();
+    return total;
+}
 
 template <class T, int RT, bool SPLIT>
-__device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const float *scale, int R, int block, float *g, float *red, RowsLds &tl) {
-    constexpr int R16 = 16 * RT, LD = RT == 1 ? 16 : R16 + 16;
+__device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const float *scale, int R, int block, float *red, int *own) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-    const int i = block / a.blocks, cb = block - i * a.blocks;
-    const int k0 = SPLIT ? cb * 64 : cb * 256 + wave * 64, k = k0 + 4 * j, left = a.K - k;
+    const int ir = block / a.blocks, cb = block - ir * a.blocks, i = ir / a.ranks, r0 = 64 * (ir - i * a.ranks);
+    const int k0 = SPLIT ? cb * 64 : cb * 256 + wave * 64, k = k0 + 4 * j;
+    int total;
+    const int *rows = own;                             // (LDS) or the sorted list's
+    if (p.perm) {
+        const int first = p.offs[i];
+        total = p.offs[i + 1] - first;
+        rows = p.perm + first;
+    } else {
+        total = p.N <= 64 ? rows_by_ballots<1>(p, i, own) : rows_by_ballots<4>(p, i, own);
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    const float f = total ? scale[i] : 0.f;
     f32x4 acc[RT][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int first = 0, total;
-    bool mine = false;
-    int place = 0;
-    if (p.perm) {
-        first = p.offs[i];
-        total = p.offs[i + 1] - first;
-    } else {
-        mine = tid < p.N && p.index[tid] == i;
-        const unsigned long long vote = __ballot(mine);
-        if (lane == 0) tl.wave_rows[wave] = __popcll(vote);
-        __syncthreads();
-        place = __popcll(vote & ((1ull << lane) - 1));
-        total = 0;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) place += tl.wave_rows[w];
-            total += tl.wave_rows[w];
+    const long long slab = (long long)p.N * a.ldp;
+    const bool whole = k0 + 64 <= a.K;                 // no lane's columns reach behind the end
+    const int stride = SPLIT ? 4 : 1, groups = (total + 15) >> 4;
+    int n[4];                                          // this lane's rows of the next group
+    auto find = [&](int group) {
+        if (group < groups)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) n[s] = rows[16 * group + 4 * s + q < total ? 16 * group + 4 * s + q : 0];
+    };
+    auto load = [&](f32x4(&x)[4], float(&g)[4][RT], int group) {
+        if (group >= groups) return;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const T *xp = a.x + n[s] * a.ldx + k;
+            if (whole) x[s] = load4(xp);
+            else x[s] = k < a.K ? load4(xp, a.K - k) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-    }
-    const float f = total ? scale[i] : 0.f;
-    for (int r0 = 0; r0 < total; r0 += 64) {
-        const int count = total - r0 < 64 ? total - r0 : 64, padded = (count + 15) & ~15;
-        __syncthreads();
-        if (p.perm) {
-            if (tid < count) tl.rows[tid] = p.perm[first + r0 + tid];
-        } else if (mine && place >= r0 && place < r0 + 64) {
-            tl.rows[place - r0] = tid;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const float *gp = a.part + (long long)n[s] * a.ldp;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) g[s][t] = gp[r0 + 16 * t + j < R ? r0 + 16 * t + j : 0];
         }
-        __syncthreads();
-        f32x4 x[4], ahead[4];                          // in flight while h is joined and while the rows before multiply
-        auto load = [&](f32x4(&v)[4], int s0) {
+        for (int sl = 1; sl < a.slices; ++sl)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const int row = s0 + 4 * s + q;
-                v[s] = row < count && left > 0 ? load4(a.x + tl.rows[row] * a.ldx + k, left) : f32x4{0.f, 0.f, 0.f, 0.f};
+                const float *gp = a.part + sl * slab + (long long)n[s] * a.ldp;
+#pragma unroll
+                for (int t = 0; t < RT; ++t) g[s][t] += gp[r0 + 16 * t + j < R ? r0 + 16 * t + j : 0];
             }
-        };
-        const int stride = SPLIT ? 64 : 16;
-        int s0 = SPLIT ? 16 * wave : 0;
-        load(x, s0);
-        for (int e = tid; e < (padded - count) * LD; e += 256) g[count * LD + e] = 0.f;
-        join<R16, LD>(g, (f32x4 *)red, a.part, a.ldp, a.slices, p.N, tl.rows, count, R, f, nullptr);
-        for (; s0 < count; s0 += stride) {
-            if (!SPLIT) load(ahead, s0 + stride);
+    };
+    auto multiply = [&](f32x4(&x)[4], float(&g)[4][RT], int group) {
+        if (16 * group + 16 > total)                   // (uniform) behind the last row: another row's values, zeros on both sides
 #pragma unroll
             for (int s = 0; s < 4; ++s)
+                if (16 * group + 4 * s + q >= total) {
+                    x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    const float gv = g[(s0 + 4 * s + q) * LD + 16 * t + j];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(gv, x[s][c], acc[t][c], 0, 0, 0);
+                    for (int t = 0; t < RT; ++t) g[s][t] = 0.f;
                 }
-            if (!SPLIT)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) x[s] = ahead[s];
-        }
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(g[s][t], x[s][c], acc[t][c], 0, 0, 0);
+    };
+    int group = SPLIT ? wave : 0;
+    find(group);
+    for (; group < groups; group += stride) {
+        f32x4 x[4];
+        float g[4][RT];
+        load(x, g, group);
+        find(group + stride);
+        multiply(x, g, group);
     }
     float *out = a.out + i * a.so;
-    if (SPLIT) {
+    auto put = [&](int r, int c, f32x4 val) {
+        if (r >= R || c >= a.K) return;
+        float *o = out + r * a.ldo + c;
+        if (a.K - c >= 4) *(f32x4_m *)o = f * val;
+        else
+            for (int y = 0; y < a.K - c; ++y) o[y] = f * val[y];
+    };
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
+    for (int t = 0; t < RT; ++t) {
+        if (SPLIT) {
             __syncthreads();
 #pragma unroll
-            for (int v = 0; v < 4; ++v) *(f32x4 *)(red + wave * 1024 + (4 * q + v) * 64 + 4 * j) = f32x4{acc[t][0][v], acc[t][1][v], acc[t][2][v], acc[t][3][v]};
+            for (int v = 0; v < 4; ++v)
+                *(f32x4 *)(red + wave * 1024 + (4 * q + v) * 64 + 4 * j) = f32x4{acc[t][0][v], acc[t][1][v], acc[t][2][v], acc[t][3][v]};
             __syncthreads();
-            const int r = 16 * t + (tid >> 4), c = cb * 64 + 4 * (tid & 15);
             const f32x4 *e = (const f32x4 *)red + tid;
-            const f32x4 val = e[0] + e[256] + e[512] + e[768];
-            if (r < R && c < a.K) {
-                float *o = out + r * a.ldo + c;
-                if (a.K - c >= 4) *(f32x4_m *)o = val;
-                else
-                    for (int y = 0; y < a.K - c; ++y) o[y] = val[y];
-            }
+            put(r0 + 16 * t + (tid >> 4), k0 + 4 * (tid & 15), (e[0] + e[256]) + (e[512] + e[768]));
+        } else {
+#pragma unroll
+            for (int v = 0; v < 4; ++v) put(r0 + 16 * t + 4 * q + v, k, f32x4{acc[t][0][v], acc[t][1][v], acc[t][2][v], acc[t][3][v]});
         }
-    } else {
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int r = 16 * t + 4 * q + v;
-                if (r >= R || left <= 0) continue;
-                float *o = out + r * a.ldo + k;
-                const f32x4 val = {acc[t][0][v], acc[t][1][v], acc[t][2][v], acc[t][3][v]};
-                if (left >= 4) *(f32x4_m *)o = val;
-                else
-                    for (int y = 0; y < left; ++y) o[y] = val[y];
-            }
     }
 }
 
 template <class T, int RT, bool SPLIT>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs<T> a, const RowsArgs<float> b, const Plan p, const float *__restrict__ scale,
                                                    int R, int a_blocks) {
-    constexpr int R16 = 16 * RT, LD = RT == 1 ? 16 : R16 + 16;
-    __shared__ RowsLds tl;
-    __shared__ __attribute__((aligned(16))) float g[64 * LD];
-    __shared__ __attribute__((aligned(16))) float red[SPLIT ? 4096 : 1024];
-    if ((int)blockIdx.x < a_blocks) rows_tile<T, RT, SPLIT>(a, p, scale, R, blockIdx.x, g, red, tl);
-    else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x - a_blocks, g, red, tl);
+    __shared__ int own[kSelfPlan];
+    __shared__ __attribute__((aligned(16))) float red[SPLIT ? 4096 : 4];
+    if ((int)blockIdx.x < a_blocks) rows_tile<T, RT, SPLIT>(a, p, scale, R, blockIdx.x, red, own);
+    else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x - a_blocks, red, own);
+}
+
+// part[0] = sum_s part[s], in order: where so many slices were needed that every reader joining them would cost more
+__global__ __launch_bounds__(256) void join_kernel(float *part, long long n4, int slices) {
+    f32x4 *p = (f32x4 *)part;
+    for (long long e = blockIdx.x * 256ll + threadIdx.x; e < n4; e += gridDim.x * 256ll) {
+        f32x4 v = p[e];
+#pragma unroll 8
+        for (int s = 1; s < slices; ++s) v += p[s * n4 + e];
+        p[e] = v;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------- the host
@@ -803,7 +848,7 @@ struct Layout {
     int rt, nt;                // ranks and rows of a tile, in 16s
     int max_tiles;
     bool sorted;               // plan_kernel's list, not each workgroup's own
-    size_t perm, offs, tiles, ntiles, part, part2, bytes;
+    size_t perm, offs, tiles, part, part2, bytes;
     int slices, slices2;       // K slices of the first contraction and, backward only, of the one that computes h again
 };
 
@@ -834,7 +879,6 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     y.perm = take(y.sorted ? 4 * (size_t)N : 0);
     y.offs = take(y.sorted ? 4 * ((size_t)L + 1) : 0);
     y.tiles = take(y.sorted ? 16 * (size_t)y.max_tiles : 0);
-    y.ntiles = take(y.sorted ? 4 : 0);
     y.part = take(64 * (size_t)y.slices * N * y.rt);
     y.part2 = take(64 * (size_t)y.slices2 * N * y.rt);
     y.bytes = at < 256 ? 256 : at;
@@ -842,18 +886,17 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
 }
 
 Plan make_plan(const Layout &y, char *ws, const int32_t *index, int N, int L, hipStream_t s) {
-    Plan p = {index, N, L, nullptr, nullptr, nullptr, nullptr};
+    Plan p = {index, N, L, nullptr, nullptr, nullptr};
     if (!y.sorted) return p;
     int waves = 15360 / (L + 1), bits = 1;             // 60 KB of counters
     waves = waves > 16 ? 16 : waves;
     while (1 << bits < L + 1) ++bits;
-    int *perm = (int *)(ws + y.perm), *offs = (int *)(ws + y.offs), *ntiles = (int *)(ws + y.ntiles);
+    int *perm = (int *)(ws + y.perm), *offs = (int *)(ws + y.offs);
     int4 *tiles = (int4 *)(ws + y.tiles);
-    plan_kernel<<<dim3(1), dim3(1024), (size_t)waves * (L + 1) * 4, s>>>(index, N, L, waves, bits, 16 * y.nt, perm, offs, tiles, ntiles);
+    plan_kernel<<<dim3(1), dim3(1024), (size_t)waves * (L + 1) * 4, s>>>(index, N, L, waves, bits, 16 * y.nt, perm, offs, tiles, y.max_tiles);
     p.perm = perm;
     p.offs = offs;
     p.tiles = tiles;
-    p.ntiles = ntiles;
     return p;
 }
 
@@ -950,33 +993,45 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
                     (((uintptr_t)x | (uintptr_t)a | (uintptr_t)b) & (sizeof(T) - 1)) == 0, "%s: pointers not aligned to their type", what);
     TY1_REQUIRE(lddz >= 0 && ldx >= 0 && lda >= 0 && sa >= 0 && ldb >= 0 && sb >= 0, "%s: negative strides", what);
     TY1_REQUIRE(apart(ldda, R, sda, L, K) && apart(lddb, R, sdb, L, U) && (!dx || apart(lddx, N, 0, 1, K)), "%s: strides make the rows of a gradient overlap", what);
-    const Layout y = layout(N, K, U, L, R, true);
+    Layout y = layout(N, K, U, L, R, true);
     TY1_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y.bytes, "%s: workspace null, not 16-byte aligned, or %zu bytes where %zu are needed", what,
                 ws_bytes, y.bytes);
-    // few adapters: 64 columns a workgroup and the rows split over its waves; enough of them: 256 columns, whole waves
-    const bool split = (long long)L * ((K + 255) / 256 + (U + 255) / 256) < 256;
-    const long long ka = split ? (K + 63ll) / 64 : (K + 255ll) / 256, ub = split ? (U + 63ll) / 64 : (U + 255ll) / 256;
-    TY1_REQUIRE(L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
+    // many rows to an adapter: they are split over the waves of a workgroup (rows_tile)
+    const bool split = N > 32ll * (L < N ? L : N);
+    const int wide = split ? 64 : 256;
+    const long long ka = (K + wide - 1ll) / wide, ub = (U + wide - 1ll) / wide;
+    TY1_REQUIRE(2 * L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
     if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 4 * ((K + 255ll) / 256)))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_backward", s, 2.0 * N * R * (K * (dx ? 2.0 : 1.0) + 2.0 * U),
                         sizeof(T) * (double)N * K + 4.0 * N * U + 4.0 * L * R * ((double)K + U) + (dx ? 4.0 * N * K : 0.0));
-    Plan p = {index, N, L, nullptr, nullptr, nullptr, nullptr};
+    Plan p = {index, N, L, nullptr, nullptr, nullptr};
     float *part = (float *)((char *)ws + y.part), *part2 = (float *)((char *)ws + y.part2);
     if (N > 0) {
         p = make_plan(y, (char *)ws, index, N, L, s);
         contract(y, p, dz, lddz, b, ldb, sb, part, U, R, y.slices, s);
-        if (!h) contract(y, p, x, ldx, a, lda, sa, part2, K, R, y.slices2, s);
+        const auto join = [&](float *sums, int &slices) {
+            if (slices == 1) return;
+            const long long n4 = 4ll * N * y.rt, blocks = (n4 + 255) / 256;
+            join_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s>>>(sums, n4, slices);
+            slices = 1;
+        };
+        if (y.sorted) join(part, y.slices);            // read by a workgroup for every 64 to 128 columns: once is worth a launch
+        if (!h) {
+            contract(y, p, x, ldx, a, lda, sa, part2, K, R, y.slices2, s);
+            join(part2, y.slices2);
+        }
     }
-    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, 16 * y.rt, (int)ka};
-    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, h ? 1 : y.slices2, h ? R : 16 * y.rt, (int)ub};
-    const dim3 grid((unsigned)(L * (ka + ub)));
+    const int ranks = y.rt == 8 ? 2 : 1;               // (128 ranks of accumulators would leave one wave a SIMD)
+    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, 16 * y.rt, (int)ka, ranks};
+    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, 1, h ? R : 16 * y.rt, (int)ub, ranks};
+    const dim3 grid((unsigned)(L * ranks * (ka + ub)));
 #define CALL(RT)                                                                                                                    \
     do {                                                                                                                            \
-        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ka));                          \
-        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ka));                               \
+        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ka));                          \
+        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ka));                               \
     } while (0)
-    if (y.rt == 1) CALL(1); else if (y.rt == 2) CALL(2); else if (y.rt == 4) CALL(4); else CALL(8);
+    if (y.rt == 1) CALL(1); else if (y.rt == 2) CALL(2); else CALL(4);
 #undef CALL
     if (dx && N > 0) expand<T>(y, p, part, y.slices, a, lda, sa, scale, dx, lddx, nullptr, K, R, 0, s);
     return ty1::check_launch(what);
