@@ -1,6 +1,8 @@
 """Thin host wrappers: torch ROCm tensors are used only as device buffers; every op below is one
 call into libty1.so (hand-written gfx950 kernels) on the current torch stream."""
 import ctypes
+import functools
+from array import array
 
 import torch
 
@@ -468,10 +470,17 @@ MAX_RANK, MAX_ADAPTERS = 128, 4096          # of ty1_adapter_*
 
 def _call_on(index, name, *args):
     """The call on device `index` and its current torch stream: the tensors' device, whatever the current one is."""
-    if index == torch.cuda.current_device():
-        return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
-    with torch.cuda.device(index):
-        return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+    return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=256)
+def _adapter_workspace_bytes(N, K, U, L, R, backward):
+    size = ctypes.c_size_t(0)
+    _lib.call('ty1_adapter_workspace_bytes', N, K, U, L, R, backward, ctypes.addressof(size))
+    return size.value
 
 
 def _strided(t, dtype, shape, index, name):
@@ -524,15 +533,14 @@ def _adapter_operands(x, a, b, index, scale):
         raise ValueError(f'{L} adapters of rank {R}: 1 to {MAX_ADAPTERS} of rank 1 to {MAX_RANK} are supported')
     if K < 1 or U < 1 or max(N, K, U) >= 2 ** 31:
         raise ValueError(f'x (N,K) = {(N, K)}, b (L,R,U) = {(L, R, U)}: sizes must be positive (N may be 0) and below 2^31')
+    if (a.dtype is x.dtype and b.dtype is x.dtype and a.get_device() == dev and b.get_device() == dev and a.shape == (L, R, K)
+            and index.dtype is torch.int32 and index.get_device() == dev and index.shape == (N,) and index.is_contiguous()
+            and scale.dtype is torch.float32 and scale.get_device() == dev and scale.shape == (L,) and scale.is_contiguous()
+            and x.stride(1) == 1 and a.stride(2) == 1 and b.stride(2) == 1):
+        return dev, N, K, U, L, R                       # the common case; what does not fit is named below, or fits after all
     _strided(x, x.dtype, (N, K), dev, 'x'); _strided(a, x.dtype, (L, R, K), dev, 'a'); _strided(b, x.dtype, (L, R, U), dev, 'b')
     _strided(index, torch.int32, (N,), dev, 'index'); _strided(scale, torch.float32, (L,), dev, 'scale')
     return dev, N, K, U, L, R
-
-
-def _adapter_workspace(x, N, K, U, L, R, backward):
-    size = ctypes.c_size_t(0)
-    _lib.call('ty1_adapter_workspace_bytes', N, K, U, L, R, backward, ctypes.addressof(size))
-    return torch.empty((size.value,), dtype=torch.uint8, device=x.device)
 
 
 def adapter_forward(x, a, b, index, scale, out=None, accumulate=False, h=None):
@@ -559,7 +567,7 @@ def adapter_forward(x, a, b, index, scale, out=None, accumulate=False, h=None):
         _chk_written(outs, [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
     if N == 0:
         return out
-    ws = _adapter_workspace(x, N, K, U, L, R, 0)
+    ws = torch.empty((_adapter_workspace_bytes(N, K, U, L, R, 0),), dtype=torch.uint8, device=x.device)
     _call_on(dev, 'ty1_adapter_forward_bf16' if x.dtype is torch.bfloat16 else 'ty1_adapter_forward_f32', x.data_ptr(), a.data_ptr(),
              b.data_ptr(), index.data_ptr(), scale.data_ptr(), out.data_ptr(), _lib.ptr(h), N, K, U, L, R, x.stride(0), a.stride(1),
              a.stride(0), b.stride(1), b.stride(0), out.stride(0), int(bool(accumulate)), ws.data_ptr(), ws.numel())
@@ -584,7 +592,7 @@ def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, 
     db = torch.empty((L, R, U), dtype=torch.float32, device=x.device) if db is None else db
     if dx is None and want_dx:
         dx = torch.empty((N, K), dtype=torch.float32, device=x.device)
-    ws = _adapter_workspace(x, N, K, U, L, R, 1)
+    ws = torch.empty((_adapter_workspace_bytes(N, K, U, L, R, 1),), dtype=torch.uint8, device=x.device)
     _call_on(dev, 'ty1_adapter_backward_bf16' if x.dtype is torch.bfloat16 else 'ty1_adapter_backward_f32', dz.data_ptr(), x.data_ptr(),
              a.data_ptr(), b.data_ptr(), index.data_ptr(), scale.data_ptr(), _lib.ptr(h), da.data_ptr(), db.data_ptr(), _lib.ptr(dx),
              N, K, U, L, R, dz.stride(0), x.stride(0), a.stride(1), a.stride(0), b.stride(1), b.stride(0), da.stride(1), da.stride(0),
@@ -594,49 +602,54 @@ def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, 
 
 def _tensor_lists(**lists):
     """One tensor or equally long lists of contiguous tensors on one GPU, float32 or bfloat16 -> (device index, n, the lists'
-    pointer arrays, value counts, types): the HOST arrays of ty1_grad_norm and its kin."""
-    names, first = list(lists), None
-    arrays = []
+    addresses, value counts, types): the HOST arrays of ty1_grad_norm and its kin, as array.array (keep them until the call)."""
+    T, first, out = torch.Tensor, None, []
     for name, ts in lists.items():
-        ts = [ts] if isinstance(ts, torch.Tensor) else list(ts)
-        lists[name] = ts
+        ts = [ts] if isinstance(ts, T) else list(ts)
+        for t in ts:
+            if not isinstance(t, T):
+                raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
         if first is None:
-            first = ts
             if not ts:
                 raise ValueError(f'{name}: no tensors')
-            for t in ts:
-                if not isinstance(t, torch.Tensor):
-                    raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
-            dev, dtypes, counts = ts[0].get_device(), [t.dtype for t in ts], [t.numel() for t in ts]
+            first, first_name, n, dev = ts, name, len(ts), ts[0].get_device()
             if dev < 0:
                 raise TypeError(f'{name}: expected tensors on the GPU (ROCm device)')
+            dtypes, shapes = [t.dtype for t in ts], [t.shape for t in ts]
             for dt in set(dtypes):
                 if dt is not torch.float32 and dt is not torch.bfloat16:
                     raise TypeError(f'{name}: expected torch.float32 or torch.bfloat16, got {dt}')
-        elif len(ts) != len(first):
-            raise ValueError(f'{name}: {len(ts)} tensors, {names[0]} has {len(first)}')
         else:
-            for t, like in zip(ts, first):
-                if not isinstance(t, torch.Tensor) or t.dtype != like.dtype:
-                    raise TypeError(f'{name}: expected tensors of the types of {names[0]}')
-                if t.shape != like.shape:
-                    raise ValueError(f'{name}: expected shape {tuple(like.shape)}, got {tuple(t.shape)}')
-        for t in ts:
-            if t.get_device() != dev:
-                raise TypeError(f'{name}: all tensors must be on GPU {dev}')
-            if not t.is_contiguous():
-                raise ValueError(f'{name}: must be contiguous')
-        arrays.append((ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]))
-    n = len(first)
-    kinds = None if torch.bfloat16 not in dtypes else (ctypes.c_int * n)(*[int(dt is torch.bfloat16) for dt in dtypes])
-    return dev, n, arrays, (ctypes.c_int64 * n)(*counts), kinds
+            if len(ts) != n:
+                raise ValueError(f'{name}: {len(ts)} tensors, {first_name} has {n}')
+            if [t.dtype for t in ts] != dtypes:
+                raise TypeError(f'{name}: expected tensors of the types of {first_name}')
+            if [t.shape for t in ts] != shapes:
+                bad = next(k for k, t in enumerate(ts) if t.shape != shapes[k])
+                raise ValueError(f'{name}: expected shape {tuple(shapes[bad])}, got {tuple(ts[bad].shape)}')
+        if {*map(T.get_device, ts)} != {dev}:
+            raise TypeError(f'{name}: all tensors must be on GPU {dev}')
+        if not all(map(T.is_contiguous, ts)):
+            raise ValueError(f'{name}: must be contiguous')
+        out.append(array('Q', map(T.data_ptr, ts)))
+    kinds = array('i', [dt is torch.bfloat16 for dt in dtypes]) if torch.bfloat16 in dtypes else None
+    return dev, n, out, array('q', map(T.numel, first)), kinds
+
+
+def _at(a):
+    return None if a is None else a.buffer_info()[0]
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_bytes(n):
+    size = ctypes.c_size_t(0)
+    _lib.call('ty1_grad_norm_workspace_bytes', n, ctypes.addressof(size))
+    return size.value
 
 
 def _norm_buffers(dev, n, norm):
-    size = ctypes.c_size_t(0)
-    _lib.call('ty1_grad_norm_workspace_bytes', n, ctypes.addressof(size))
     device = torch.device('cuda', dev)
-    ws = torch.empty((size.value,), dtype=torch.uint8, device=device)
+    ws = torch.empty((_norm_workspace_bytes(n),), dtype=torch.uint8, device=device)
     return ws, torch.empty((1,), dtype=torch.float32, device=device) if norm is None else _chk_out(norm, torch.float32, (1,), 'norm')
 
 
@@ -652,7 +665,7 @@ def grad_norm(grads, norm=None):
     the device: squares and sums in float64, in an order fixed by the sizes.  norm: optional (1,) buffer."""
     dev, n, (g,), counts, kinds = _tensor_lists(grads=grads)
     ws, norm = _norm_buffers(dev, n, norm)
-    _call_on(dev, 'ty1_grad_norm', g, counts, kinds, n, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    _call_on(dev, 'ty1_grad_norm', _at(g), _at(counts), _at(kinds), n, norm.data_ptr(), ws.data_ptr(), ws.numel())
     return norm
 
 
@@ -663,7 +676,7 @@ def clip_grad_norm(grads, max_norm, out=None, norm=None):
     max_norm = _max_norm(max_norm)
     dev, n, arrays, counts, kinds = _tensor_lists(grads=grads, out=out) if out is not None else _tensor_lists(grads=grads)
     ws, norm = _norm_buffers(dev, n, norm)
-    _call_on(dev, 'ty1_clip_grad_norm', arrays[0], arrays[-1], counts, kinds, n, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    _call_on(dev, 'ty1_clip_grad_norm', _at(arrays[0]), _at(arrays[-1]), _at(counts), _at(kinds), n, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel())
     return norm
 
 
@@ -678,7 +691,7 @@ def adam_step_clipped(p, g, m, v, t, max_norm, lr=1e-3, beta1=0.9, beta2=0.999, 
     if kinds is not None:
         raise TypeError('p, g, m, v: expected torch.float32')
     ws, norm = _norm_buffers(dev, n, norm)
-    _call_on(dev, 'ty1_adam_step_clip_f32', pp, gg, mm, vv, counts, n, max_norm, float(lr), float(beta1), float(beta2), float(eps),
+    _call_on(dev, 'ty1_adam_step_clip_f32', _at(pp), _at(gg), _at(mm), _at(vv), _at(counts), n, max_norm, float(lr), float(beta1), float(beta2), float(eps),
              int(t), norm.data_ptr(), ws.data_ptr(), ws.numel())
     return norm
 
