@@ -600,7 +600,7 @@ struct ExpandArgs {
 };
 
 template <class T, int NT, int RT>
-__global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, const Plan p) {
+__global__ __launch_bounds__(256, RT <= 2 || NT * RT == 4 ? 3 : 1) void expand_kernel(const ExpandArgs<T> a, const Plan p) {
     constexpr int TM = 16 * NT, R16 = 16 * RT, LD = R16 + 4, STEPS = R16 / 4;
     __shared__ TileLds tl;
     __shared__ __attribute__((aligned(16))) float h[TM * LD];
@@ -628,11 +628,17 @@ __global__ __launch_bounds__(256) void expand_kernel(const ExpandArgs<T> a, cons
     int u = first * 256 + wave * 64 + 4 * j;
     const T *mp = a.m + adapter * a.sm;
     auto load = [&](f32x4 *v, int c) {
+        if (c - 4 * j + 64 <= a.U) {                   // (uniform) all of the wave's columns are there
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-            const int r = q * STEPS + k;
-            v[k] = r < a.R && c < a.U ? load4(mp + r * a.ldm + c, a.U - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < STEPS; ++k) v[k] = load4(mp + (q * STEPS + k < a.R ? q * STEPS + k : 0) * a.ldm + c);
+        } else {
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) v[k] = c < a.U ? load4(mp + (q * STEPS + k < a.R ? q * STEPS + k : 0) * a.ldm + c, a.U - c) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        if (a.R < R16)                                 // ranks that are not there: zeros on both sides
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                if (q * STEPS + k >= a.R) v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
     load(m, u);
     for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
@@ -946,6 +952,13 @@ void expand(const Layout &y, const Plan &p, const float *part, int slices, const
 #undef CALL
 }
 
+void join_slices(const Layout &y, float *part, int &slices, int N, hipStream_t s) {
+    if (slices == 1) return;
+    const long long n4 = 4ll * N * y.rt, blocks = (n4 + 255) / 256;
+    join_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s>>>(part, n4, slices);
+    slices = 1;
+}
+
 // a tensor that is written: its rows must not overlap
 bool apart(int64_t ld, int rows, int64_t stride, int slabs, int cols) {
     if (rows > 1 && ld < cols) return false;
@@ -1010,16 +1023,10 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     if (N > 0) {
         p = make_plan(y, (char *)ws, index, N, L, s);
         contract(y, p, dz, lddz, b, ldb, sb, part, U, R, y.slices, s);
-        const auto join = [&](float *sums, int &slices) {
-            if (slices == 1) return;
-            const long long n4 = 4ll * N * y.rt, blocks = (n4 + 255) / 256;
-            join_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, s>>>(sums, n4, slices);
-            slices = 1;
-        };
-        if (y.sorted) join(part, y.slices);            // read by a workgroup for every 64 to 128 columns: once is worth a launch
+        if (y.sorted) join_slices(y, part, y.slices, N, s);       // read by a workgroup for every 64 columns: once is worth a launch
         if (!h) {
             contract(y, p, x, ldx, a, lda, sa, part2, K, R, y.slices2, s);
-            join(part2, y.slices2);
+            join_slices(y, part2, y.slices2, N, s);
         }
     }
     const int ranks = y.rt == 8 ? 2 : 1;               // (128 ranks of accumulators would leave one wave a SIMD)
