@@ -98,31 +98,53 @@ class DeviceModel:
         return (self.dtype == 'bf16' and len(s) >= 2 and tuple(s[0]) == (3, 16, True) and tuple(s[1]) == (16, 32, True)
                 and x.shape[1] % 4 == 0 and x.shape[2] % 4 == 0 and 0.0 < LEAKY_ALPHA <= 1.0)
 
-    def head(self, feats, ws=None):
+    def dense(self, feats, ws=None, adapters=None, index=None, h=None):
+        """Split-K partials (splits,N,ldz) of the Dense layer for the kernels behind it.  adapters (adapters.AdapterBank) and
+        index (N) int32 on the device (AdapterBank.index; -1: none): image n goes through the Dense layer plus adapter index[n],
+        whose product is one more partial, summed by whatever kernel reduces the others.  h: see ops.adapter_forward."""
         ws = ws or self.workspace(feats.shape[0])
         wt = self.dense_wt_bf16 if self.dtype == 'bf16' else self.dense_wt
-        part = ops.dense_splitk(feats, wt, self.units, part=ws['part'])
+        if adapters is None:
+            if index is not None:
+                raise ValueError('index without adapters')
+            return ops.dense_splitk(feats, wt, self.units, part=ws['part'])
+        if index is None:
+            raise ValueError('adapters need an index: one adapter per image, -1 for none')
+        if (adapters.features, adapters.units) != (self.K, self.units):
+            raise ValueError(f'adapters of a {adapters.features} x {adapters.units} Dense layer do not fit {self.K} x {self.units}')
+        part = ws.get('part_adapted')
+        if part is None:
+            splits, N, ldz = ws['part'].shape
+            part = ws['part_adapted'] = torch.empty((splits + 1, N, ldz), dtype=torch.float32, device=self.device)
+        ops.dense_splitk(feats, wt, self.units, part=part[:-1])
+        a, b = adapters.weights(feats.dtype)
+        ops.adapter_forward(feats, a, b, index, adapters.scale, out=part[-1][:, :self.units], h=h)
+        return part
+
+    def head(self, feats, ws=None, adapters=None, index=None):
+        ws = ws or self.workspace(feats.shape[0])
+        part = self.dense(feats, ws, adapters, index)
         return ops.head_activate(part, self.dense_b, self.S, self.B, self.C, out=ws['y'])
 
-    def predict(self, x):
-        """-> y_pred (N,S,S,C+5B) on the device (valid until the next call with the same N).
+    def predict(self, x, adapters=None, index=None):
+        """-> y_pred (N,S,S,C+5B) on the device (valid until the next call with the same N); adapters, index: see dense().
         With a Trainer attached: an update left in flight by step(wait=False) must be joined first (Trainer.join()),
         otherwise this forward reads the weights from before it.  The same holds for detect()."""
         ws = self.workspace(x.shape[0])
-        return self.head(self.backbone(x, ws), ws)
+        return self.head(self.backbone(x, ws), ws, adapters, index)
 
     FUSED_TAIL_MIN_BATCH = 1       # (with 85 Dense splits the two-launch tail won below 16 images; with 21 the fused one wins from 1)
 
-    def detect(self, x, iou_thr=0.2, want_y=False):
+    def detect(self, x, iou_thr=0.2, want_y=False, adapters=None, index=None):
         """-> (boxes f64 (N,S*S*B,4), score, cls, keep) on the device.  From FUSED_TAIL_MIN_BATCH images on, everything
-        behind the Dense GEMM is one launch (ty1_head_decode_nms_f32) and the head tensor stays in LDS unless want_y."""
+        behind the Dense GEMM is one launch (ty1_head_decode_nms_f32) and the head tensor stays in LDS unless want_y.
+        adapters, index: see dense()."""
         N = x.shape[0]
         ws = self.workspace(N)
         feats = self.backbone(x, ws)
         if N < self.FUSED_TAIL_MIN_BATCH:
-            return ops.decode_nms(self.head(feats, ws), self.B, self.C, self.img_size, iou_thr, out=ws['det'])
-        wt = self.dense_wt_bf16 if self.dtype == 'bf16' else self.dense_wt
-        part = ops.dense_splitk(feats, wt, self.units, part=ws['part'])
+            return ops.decode_nms(self.head(feats, ws, adapters, index), self.B, self.C, self.img_size, iou_thr, out=ws['det'])
+        part = self.dense(feats, ws, adapters, index)
         return ops.head_decode_nms(part, self.dense_b, self.S, self.B, self.C, self.img_size, iou_thr,
                                    y=ws['y'] if want_y else None, out=ws['det'])
 
@@ -234,7 +256,9 @@ class Trainer:
 
     UPDATE_AFTER_LAYER = 2        # 112x112x32->64: in-call A/B tools/experiments/tail_side_ab.sh at 32 images (ms per step): at once 0.977, after layer 0 / 1 / 2 / 3 / 4 / 5: 0.979 / 1.004 / 0.971 / 0.977 / 0.973 / 0.988
 
-    def __init__(self, model, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, group=None, overlap=True):
+    def __init__(self, model, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, group=None, overlap=True, global_clipnorm=None):
+        """global_clipnorm: clip the group's summed gradient to this global norm before Adam (Keras' Adam(global_clipnorm=...));
+        the norm before clipping is left in self.grad_norm (1,) on the device, ordered like the update."""
         if model.dtype != 'f32':
             raise ValueError("training runs in fp32 (the reference's arithmetic): build the model with dtype='f32'")
         from . import parallel
@@ -253,6 +277,8 @@ class Trainer:
         model._graphs.clear()            # captured graphs hold the old parameter addresses
         self.m, self.v = torch.zeros_like(self.pflat), torch.zeros_like(self.pflat)
         self.t = 0
+        self.global_clipnorm = None if global_clipnorm is None else ops._max_norm(global_clipnorm)
+        self.grad_norm = torch.zeros((1,), dtype=torch.float32, device=dev)
         self.ldz = ops.round_up(model.units, 4)
         self._dz = {}
         self.side = torch.cuda.Stream(dev) if overlap else None
@@ -386,6 +412,10 @@ class Trainer:
 
     def _adam(self):
         self.t += 1
+        if self.global_clipnorm is not None:       # one more read of the gradient; the clipped values never reach memory
+            ops.adam_step_clipped(self.pflat, self.bucket.grads, self.m, self.v, self.t, self.global_clipnorm, self.lr, self.beta1,
+                                  self.beta2, self.eps, norm=self.grad_norm)
+            return
         ops.adam_step(self.pflat, self.bucket.grads, self.m, self.v, self.t, self.lr, self.beta1, self.beta2, self.eps)
 
     def _exchange_and_update(self, defer_adam=False, loss_out=None):
@@ -481,3 +511,56 @@ class Trainer:
         if wait:
             self.join()
         return losses
+
+
+class AdapterTrainer:
+    """Training of an AdapterBank with the backbone AND the shared Dense layer frozen: batches mix images of any adapters, every
+    adapter learns from its own images, and one Adam (Keras defaults) updates the whole bank, clipped by the global norm over
+    all adapters where global_clipnorm is given.  The loss is the batch sum of yolo_loss (/root/reference/yolo/yolo.py:48-107)
+    and data parallelism exchanges one flat buffer [dA | dB | loss] by SUM, as Trainer does.  Adapters without images in a step
+    get a zero gradient; their moments decay and may still move them, as Keras' dense Adam does.  Everything runs in order on
+    the caller's stream."""
+
+    def __init__(self, model, bank, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, group=None, global_clipnorm=None):
+        if model.dtype != 'f32':
+            raise ValueError("training runs in fp32 (the reference's arithmetic): build the model with dtype='f32'")
+        if (bank.features, bank.units, bank.device) != (model.K, model.units, model.device):
+            raise ValueError(f'the bank is for a {bank.features} x {bank.units} Dense layer on {bank.device}')
+        self.model, self.bank, self.group = model, bank, group
+        self.lr, self.beta1, self.beta2, self.eps = lr, beta1, beta2, eps
+        self.global_clipnorm = None if global_clipnorm is None else ops._max_norm(global_clipnorm)
+        n = bank.flat.numel()
+        self.bucket = torch.zeros(n + 1, dtype=torch.float32, device=model.device)
+        self.grads, self.loss = self.bucket[:n], self.bucket[n:]
+        self.da, self.db = bank.views(self.grads)
+        self.m, self.v = torch.zeros_like(bank.flat), torch.zeros_like(bank.flat)
+        self.t = 0
+        self.ldz = ops.round_up(model.units, 4)
+        self.grad_norm = torch.zeros((1,), dtype=torch.float32, device=model.device)
+
+    def gradients(self, x, y_true, index):
+        """Forward + backward on this rank's images: fills self.da / self.db, returns the local loss (1,) (a view)."""
+        return self.gradients_from_features(self.model.backbone(x, self.model.workspace(x.shape[0])), y_true, index)
+
+    def gradients_from_features(self, feats, y_true, index):
+        m, bank, N = self.model, self.bank, feats.shape[0]
+        h = torch.empty((N, bank.rank), dtype=torch.float32, device=m.device)
+        part = m.dense(feats, m.workspace(N), bank, index, h=h)
+        _, _, dz = ops.train_tail(part, m.dense_b, y_true, self.ldz, m.S, m.B, m.C, m.img_size, loss_out=self.loss)
+        ops.adapter_backward(dz[:, :m.units], feats, bank.a, bank.b, index, bank.scale, h, da=self.da, db=self.db)
+        return self.loss
+
+    def step(self, x, y_true, index):
+        """x (n,H,W,3), y_true (n,S,S,C+5), index (n) int32 (AdapterBank.index) on the device -> the group's batch loss (1,)."""
+        from . import parallel
+        self.gradients(x, y_true, index)
+        parallel.allreduce_flat(self.bucket, self.group)
+        loss = self.loss.clone()
+        self.t += 1
+        if self.global_clipnorm is not None:
+            ops.adam_step_clipped(self.bank.flat, self.grads, self.m, self.v, self.t, self.global_clipnorm, self.lr, self.beta1,
+                                  self.beta2, self.eps, norm=self.grad_norm)
+        else:
+            ops.adam_step(self.bank.flat, self.grads, self.m, self.v, self.t, self.lr, self.beta1, self.beta2, self.eps)
+        self.bank.changed()
+        return loss

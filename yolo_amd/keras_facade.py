@@ -87,9 +87,13 @@ class Dense(Layer):
 
 
 class Adam:
-    """tensorflow.keras.optimizers.Adam(lr=0.001) with Keras defaults (train.py:59)."""
+    """tensorflow.keras.optimizers.Adam(lr=0.001) with Keras defaults (train.py:59).  global_clipnorm: Keras' argument of that
+    name, the gradients of all trainable weights are scaled down together to this norm."""
 
-    def __init__(self, lr=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-7, learning_rate=None):
+    def __init__(self, lr=0.001, beta_1=0.9, beta_2=0.999, epsilon=1e-7, learning_rate=None, global_clipnorm=None):
+        if global_clipnorm is not None and not float(global_clipnorm) > 0:
+            raise ValueError(f'global_clipnorm must be positive, got {global_clipnorm}')
+        self.global_clipnorm = global_clipnorm
         self.lr = learning_rate if learning_rate is not None else lr
         self.beta_1, self.beta_2, self.epsilon = beta_1, beta_2, epsilon
 
@@ -267,7 +271,7 @@ class Model:
         if self._trainer is None:
             from .engine import Trainer
             o = self.optimizer or Adam()
-            self._trainer = Trainer(self.engine, o.lr, o.beta_1, o.beta_2, o.epsilon, group)
+            self._trainer = Trainer(self.engine, o.lr, o.beta_1, o.beta_2, o.epsilon, group, global_clipnorm=getattr(o, 'global_clipnorm', None))
         return self._trainer
 
     def train_on_batch(self, x, y):

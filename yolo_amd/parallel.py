@@ -30,6 +30,19 @@ def allreduce_sum_(tensors, group=None):
     return tensors
 
 
+def allreduce_flat(flat, group=None):
+    """In-place SUM all-reduce of one flat buffer, ordered on the current stream; nothing for a single rank.  A backend other than
+    'nccl' (the gloo rehearsals) gets a host copy of a device buffer."""
+    if world(group)[1] == 1:
+        return flat
+    if flat.is_cuda and dist.get_backend(group) != 'nccl':
+        host = flat.cpu()
+        dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+        return flat.copy_(host)
+    dist.all_reduce(flat, op=dist.ReduceOp.SUM, group=group)
+    return flat
+
+
 class GradBucket:
     """The training step's one exchange: Dense weight gradient, bias gradient and the batch loss live in ONE
     contiguous fp32 buffer [dWt (rows x ldk) | db (units) | loss (1)], so a step issues a single SUM all-reduce
