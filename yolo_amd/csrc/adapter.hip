@@ -560,12 +560,12 @@ __device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ pa
             const int row = e / R16, r = e % R16;
             dst[row * LD + r] = r < R ? f * part[(long long)rows[row] * ldp + r] : 0.f;
         }
-    } else if (N * R4 <= 64 && slices > 4) {          // a small batch: several threads to a value, as many for every tile
-        const int n = N * R4, groups = 256 / n, e = tid % n, g = tid / n, row = e / R4, r = 4 * (e % R4);
+    } else if (slices > 4 && N * R4 <= 64) {           // a batch of few values: 4 to 8 threads to a value, as many for every tile
+        const int n = N * R4, most = 256 / n, groups = most < 8 ? most : 8, e = tid % n, g = tid / n, row = e / R4, r = 4 * (e % R4);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (g < groups && row < count) {
             const float *src = part + (long long)rows[row] * ldp + r;
-#pragma unroll 4
+#pragma unroll 8
             for (int s = g; s < slices; s += groups) v += *(const f32x4_m *)(src + s * slab);
         }
         lds[tid] = v;
@@ -823,11 +823,11 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
 
 template <class T, int RT, bool SPLIT>
 __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs<T> a, const RowsArgs<float> b, const Plan p, const float *__restrict__ scale,
-                                                   int R, int a_blocks) {
+                                                   int R, int b_blocks) {
     __shared__ int own[kSelfPlan];
     __shared__ __attribute__((aligned(16))) float red[SPLIT ? 4096 : 4];
-    if ((int)blockIdx.x < a_blocks) rows_tile<T, RT, SPLIT>(a, p, scale, R, blockIdx.x, red, own);
-    else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x - a_blocks, red, own);
+    if ((int)blockIdx.x >= b_blocks) rows_tile<T, RT, SPLIT>(a, p, scale, R, blockIdx.x - b_blocks, red, own);
+    else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x, red, own);          // (fewer: a long one last would be waited for)
 }
 
 // part[0] = sum_s part[s], in order: where so many slices were needed that every reader joining them would cost more
@@ -858,10 +858,9 @@ struct Layout {
     int slices, slices2;       // K slices of the first contraction and, backward only, of the one that computes h again
 };
 
-int slices_for(int tiles, int K) {
-    // enough workgroups for every CU to hold four, but at least 512 elements of K for a workgroup (128 a wave: below that the
-    // join of the slices costs more than their reading)
-    const int want = (4 * 256 + tiles - 1) / tiles, most = (K + 511) / 512;
+int slices_for(int tiles, int K, int least) {
+    // enough workgroups for every CU to hold four, but at least `least` elements of K for a workgroup
+    const int want = (4 * 256 + tiles - 1) / tiles, most = (K + least - 1) / least;
     const int s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : s;
 }
@@ -874,8 +873,10 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     const long long tiles = (long long)N / (16 * y.nt) + (L + 1 < N ? L + 1 : N);
     y.max_tiles = (int)(tiles < N ? tiles : N > 1 ? N : 1);
     y.sorted = N > kSelfPlan;
-    y.slices = back ? slices_for(y.max_tiles, U) : slices_for(y.max_tiles, K);
-    y.slices2 = back ? slices_for(y.max_tiles, K) : 0;
+    // Slices that every reader joins by itself: 512 elements (256 make one frame's contraction 0.7 us faster and what reads it
+    // 1 us slower).  Joined by a launch of their own: 256 (2048 rows x 1470 of rank 32: 12.5 -> 10.2 us).
+    y.slices = slices_for(y.max_tiles, back ? U : K, back && y.sorted ? 256 : 512);
+    y.slices2 = back ? slices_for(y.max_tiles, K, 256) : 0;
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -1035,8 +1036,8 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     const dim3 grid((unsigned)(L * ranks * (ka + ub)));
 #define CALL(RT)                                                                                                                    \
     do {                                                                                                                            \
-        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ka));                          \
-        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ka));                               \
+        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ub));                          \
+        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ub));                               \
     } while (0)
     if (y.rt == 1) CALL(1); else if (y.rt == 2) CALL(2); else CALL(4);
 #undef CALL

@@ -2,6 +2,7 @@
 call into libty1.so (hand-written gfx950 kernels) on the current torch stream."""
 import ctypes
 import functools
+import operator
 from array import array
 
 import torch
@@ -468,12 +469,16 @@ def adam_step(p, g, m, v, t, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7):
 MAX_RANK, MAX_ADAPTERS = 128, 4096          # of ty1_adapter_*
 
 
+# the handle of a device's current stream: the call behind torch.cuda.current_stream(i).cuda_stream without the Stream object (1 us)
+_stream_of = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call_on(index, name, *args):
     """The call on device `index` and its current torch stream: the tensors' device, whatever the current one is."""
     if index != torch.cuda.current_device():
         with torch.cuda.device(index):
-            return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
-    return _lib.call(name, *args, torch.cuda.current_stream(index).cuda_stream)
+            return _lib.call(name, *args, _stream_of(index))
+    return _lib.call(name, *args, _stream_of(index))
 
 
 @functools.lru_cache(maxsize=256)
@@ -583,10 +588,12 @@ def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, 
     dev, N, K, U, L, R = _adapter_operands(x, a, b, index, scale)
     _strided(dz, torch.float32, (N, U), dev, 'dz')
     if h is not None:
-        _chk_out(_strided(h, torch.float32, (N, R), dev, 'h'), torch.float32, (N, R), 'h')
-    given = [(name, _strided(t, torch.float32, shape, dev, name)) for name, t, shape in
-             (('da', da, (L, R, K)), ('db', db, (L, R, U)), ('dx', dx, (N, K))) if t is not None]
-    if given:
+        _strided(h, torch.float32, (N, R), dev, 'h')
+        if not h.is_contiguous():
+            raise ValueError('h: must be contiguous')
+    if da is not None or db is not None or dx is not None:
+        given = [(name, _strided(t, torch.float32, shape, dev, name)) for name, t, shape in
+                 (('da', da, (L, R, K)), ('db', db, (L, R, U)), ('dx', dx, (N, K))) if t is not None]
         _chk_written(given, [('dz', dz), ('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)] + ([('h', h)] if h is not None else []))
     da = torch.empty((L, R, K), dtype=torch.float32, device=x.device) if da is None else da
     db = torch.empty((L, R, U), dtype=torch.float32, device=x.device) if db is None else db
@@ -600,40 +607,43 @@ def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, 
     return da, db, dx
 
 
+_DTYPE = operator.attrgetter('dtype')
+
+
 def _tensor_lists(**lists):
-    """One tensor or equally long lists of contiguous tensors on one GPU, float32 or bfloat16 -> (device index, n, the lists'
-    addresses, value counts, types): the HOST arrays of ty1_grad_norm and its kin, as array.array (keep them until the call)."""
+    """One tensor or equally long lists of contiguous tensors on one GPU, float32 or bfloat16, with as many values list by list ->
+    (device index, n, the lists' addresses, value counts, types): the HOST arrays of ty1_grad_norm and its kin, as array.array
+    (keep them until the call)."""
     T, first, out = torch.Tensor, None, []
     for name, ts in lists.items():
         ts = [ts] if isinstance(ts, T) else list(ts)
-        for t in ts:
-            if not isinstance(t, T):
-                raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
+        for kind in {*map(type, ts)}:
+            if not issubclass(kind, T):
+                raise TypeError(f'{name}: expected tensors, got {kind.__name__}')
         if first is None:
             if not ts:
                 raise ValueError(f'{name}: no tensors')
-            first, first_name, n, dev = ts, name, len(ts), ts[0].get_device()
+            first, n, dev, dtypes, counts = name, len(ts), ts[0].get_device(), [*map(_DTYPE, ts)], [*map(T.numel, ts)]
             if dev < 0:
                 raise TypeError(f'{name}: expected tensors on the GPU (ROCm device)')
-            dtypes, shapes = [t.dtype for t in ts], [t.shape for t in ts]
-            for dt in set(dtypes):
+            for dt in {*dtypes}:
                 if dt is not torch.float32 and dt is not torch.bfloat16:
                     raise TypeError(f'{name}: expected torch.float32 or torch.bfloat16, got {dt}')
         else:
             if len(ts) != n:
-                raise ValueError(f'{name}: {len(ts)} tensors, {first_name} has {n}')
-            if [t.dtype for t in ts] != dtypes:
-                raise TypeError(f'{name}: expected tensors of the types of {first_name}')
-            if [t.shape for t in ts] != shapes:
-                bad = next(k for k, t in enumerate(ts) if t.shape != shapes[k])
-                raise ValueError(f'{name}: expected shape {tuple(shapes[bad])}, got {tuple(ts[bad].shape)}')
+                raise ValueError(f'{name}: {len(ts)} tensors, {first} has {n}')
+            if [*map(_DTYPE, ts)] != dtypes:
+                raise TypeError(f'{name}: expected tensors of the types of {first}')
+            if [*map(T.numel, ts)] != counts:
+                bad = next(k for k, t in enumerate(ts) if t.numel() != counts[k])
+                raise ValueError(f'{name}: tensor {bad} has {ts[bad].numel()} values, in {first} it has {counts[bad]}')
         if {*map(T.get_device, ts)} != {dev}:
             raise TypeError(f'{name}: all tensors must be on GPU {dev}')
         if not all(map(T.is_contiguous, ts)):
             raise ValueError(f'{name}: must be contiguous')
         out.append(array('Q', map(T.data_ptr, ts)))
     kinds = array('i', [dt is torch.bfloat16 for dt in dtypes]) if torch.bfloat16 in dtypes else None
-    return dev, n, out, array('q', map(T.numel, first)), kinds
+    return dev, n, out, array('q', counts), kinds
 
 
 def _at(a):
@@ -671,7 +681,7 @@ def grad_norm(grads, norm=None):
 
 def clip_grad_norm(grads, max_norm, out=None, norm=None):
     """Scales one tensor or a list of tensors by min(1, max_norm / global norm), in place or into out (as many tensors of the
-    same shapes and types) -> the norm before clipping, (1,) float32 on the device.  A norm that is not finite makes every
+    same numbers of values and types) -> the norm before clipping, (1,) float32 on the device.  A norm that is not finite makes every
     value NaN (Keras' global_clipnorm, tf.clip_by_global_norm).  Tensors must not overlap one another."""
     max_norm = _max_norm(max_norm)
     dev, n, arrays, counts, kinds = _tensor_lists(grads=grads, out=out) if out is not None else _tensor_lists(grads=grads)
