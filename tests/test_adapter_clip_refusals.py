@@ -33,7 +33,7 @@ def _refused(name, args, text):
 
 @pytest.mark.parametrize('suffix', ['f32', 'bf16'])
 @pytest.mark.parametrize('kw, text', [
-    (dict(N=-1), 'bad dimensions'), (dict(K=0), 'bad dimensions'), (dict(U=0), 'bad dimensions'),
+    (dict(N=-1), 'bad dimensions'), (dict(N=(1 << 30) + 1), 'bad dimensions'), (dict(K=0), 'bad dimensions'), (dict(U=0), 'bad dimensions'),
     (dict(L=0), '0 adapters'), (dict(L=4097), '4097 adapters'), (dict(R=0), 'rank 0'), (dict(R=129), 'rank 129'),
     (dict(x=None), 'null pointer'), (dict(b=None), 'null pointer'), (dict(index=None), 'null pointer'), (dict(scale=None), 'null pointer'),
     (dict(x=P + 1), 'not aligned'), (dict(scale=P + 2), 'not aligned'), (dict(ldx=-8), 'negative strides'), (dict(sb=-1), 'negative strides'),
@@ -83,10 +83,10 @@ def test_clip_calls_refused():
         _refused('ty1_grad_norm', args, text)
     for args, text in (((g, o, c, None, 2, 0.0, P, P, *big), 'must be positive'), ((g, o, c, None, 2, -1.0, P, P, *big), 'must be positive'),
                        ((g, o, c, None, 2, float('nan'), P, P, *big), 'must be positive'), ((g, None, c, None, 2, 1.0, P, P, *big), 'null list'),
-                       ((g, _ptrs(P + 4, P + 8192), c, None, 2, 1.0, P, P, *big), 'shares memory'),          # shifted onto itself
-                       ((g, _ptrs(P + 8192, P + 8196), c, None, 2, 1.0, P, P, *big), 'shares memory'),       # outputs on one another
-                       ((g, _ptrs(P + 4096, P), _i64s(8, 8), None, 2, 1.0, P, P, *big), 'shares memory'),    # crosswise
-                       ((_ptrs(P, P), _ptrs(P, P), _i64s(8, 8), None, 2, 1.0, P, P, *big), 'shares memory'),  # one tensor twice
+                       ((g, _ptrs(P + 4, P + 8192), c, None, 2, 1.0, 0x8000, P, *big), 'shares memory'),          # shifted onto itself
+                       ((g, _ptrs(P + 8192, P + 8196), c, None, 2, 1.0, 0x8000, P, *big), 'shares memory'),       # outputs on one another
+                       ((g, _ptrs(P + 4096, P), _i64s(8, 8), None, 2, 1.0, 0x8000, P, *big), 'shares memory'),    # crosswise
+                       ((_ptrs(P, P), _ptrs(P, P), _i64s(8, 8), None, 2, 1.0, 0x8000, P, *big), 'shares memory'),  # one tensor twice
                        ((g, o, c, None, 2, 1.0, P, P, 8, None), 'workspace')):
         _refused('ty1_clip_grad_norm', args, text)
 
@@ -94,13 +94,16 @@ def test_clip_calls_refused():
 def test_clipped_adam_calls_refused():
     lists = [_ptrs(P + 65536 * l, P + 65536 * l + 8192) for l in range(4)]
     c = _i64s(1000, 8)
-    tail = (1e-3, 0.9, 0.999, 1e-7, 1, P, P, 1 << 24, None)
+    tail = (1e-3, 0.9, 0.999, 1e-7, 1, 0x8000, P, 1 << 24, None)
     _refused('ty1_adam_step_clip_f32', (*lists, c, 0, 1.0, *tail), 'no tensors')
     _refused('ty1_adam_step_clip_f32', (*lists, c, 2, 0.0, *tail), 'must be positive')
     _refused('ty1_adam_step_clip_f32', (*lists, c, 2, 1.0, 1e-3, 0.9, 0.999, 1e-7, 0, P, P, 1 << 24, None), 'bad t=0')
     _refused('ty1_adam_step_clip_f32', (lists[0], lists[0], *lists[2:], c, 2, 1.0, *tail), 'shares memory')
     _refused('ty1_adam_step_clip_f32', (*lists[:3], lists[2], c, 2, 1.0, *tail), 'shares memory')
     _refused('ty1_adam_step_clip_f32', (*lists, c, 2, 1.0, 1e-3, 0.9, 0.999, 1e-7, 1, None, P, 1 << 24, None), 'null pointer')
+    for betas in ((1.0, 0.999), (0.9, 1.0), (-0.1, 0.999), (0.9, float('nan'))):
+        _refused('ty1_adam_step_clip_f32', (*lists, c, 2, 1.0, 1e-3, *betas, 1e-7, 1, 0x8000, P, 1 << 24, None), 'betas')
+    _refused('ty1_adam_step_clip_f32', (*lists, c, 2, 1.0, 1e-3, 0.9, 0.999, 1e-7, 1, P + 3996, P, 1 << 24, None), 'shares memory')   # the norm in p
 
 
 def test_ops_refuse_host_tensors():

@@ -111,6 +111,53 @@ def test_real_values_within_the_bound(N, K, U, L, R, dtype):
     _close(dx, want['dx'], mag['dx'], U, R, 'dx')
 
 
+# the variants that take long batches or long axes: contraction through LDS in its three type mixtures and all tile shapes, 64 and
+# 32 rows a workgroup and several column blocks in the expansion, 128 ranks in halves, thousands of adapters
+LONG = [(4000, 9001, 33, 2, 64, torch.float32), (2100, 9003, 20, 1, 100, torch.float32), (4000, 9001, 18, 3, 20, torch.float32),
+        (4000, 9001, 35, 3, 9, torch.float32), (4000, 16500, 20, 2, 40, torch.bfloat16), (4000, 40, 9001, 2, 30, torch.bfloat16),
+        (4000, 40, 9001, 2, 61, torch.bfloat16), (2100, 30, 9002, 1, 128, torch.bfloat16), (4000, 64, 4100, 2, 17, torch.float32),
+        (40, 100, 50, 5, 100, torch.float32), (600, 20, 16, 4096, 3, torch.float32), (256, 40, 20, 4096, 2, torch.bfloat16),
+        (257, 513, 1025, 1, 1, torch.float32)]
+
+
+@pytest.mark.parametrize('N, K, U, L, R, dtype', LONG)
+def test_long_batches_exact(N, K, U, L, R, dtype):
+    x, a, b, index, scale, dz = _inputs(N, K, U, L, R, dtype, N + U, whole=True, none=0.05)
+    # one value in eight of x and dz, so that the longest sums stay below 2^24 quarters (the smallest scale): asserted
+    g = torch.Generator().manual_seed(N)
+    x, dz = x * (torch.rand(x.shape, generator=g) < 0.125).to(DEV), dz.sign() * (torch.rand(dz.shape, generator=g) < 0.125).to(DEV)
+    want, mag = _formula(x, a, b, index, scale, dz)
+    assert max(float(m.max()) for m in mag.values()) < 2 ** 24 * 0.25
+    h = torch.empty((N, R), device=DEV)
+    _equal(ops.adapter_forward(x, a, b, index, scale, h=h), want['out'], 'out')
+    _equal(h, want['h'], 'h')
+    for kept in (h, None):
+        da, db, dx = ops.adapter_backward(dz, x, a, b, index, scale, kept, want_dx=True)
+        _equal(da, want['da'], 'da'); _equal(db, want['db'], 'db'); _equal(dx, want['dx'], 'dx')
+
+
+def test_offsets_beyond_32_bits():
+    """Rows, adapters and outputs 1.1e9 elements apart in buffers of 9 GB: element offsets above 2^31, byte offsets above 2^32."""
+    far, N, K, U, L, R = 1_100_000_000, 3, 70, 40, 3, 5
+    xs, as_, bs, index, scale, dzs = _inputs(N, K, U, L, R, torch.float32, 6, whole=True, none=0.0)
+    index = torch.tensor([2, 0, 2], dtype=torch.int32, device=DEV)
+    ins, outs = (torch.empty(2 * far + 4096, device=DEV) for _ in range(2))
+    view = lambda buf, shape, at: buf.as_strided(shape, (far,) + ((shape[2],) if len(shape) == 3 else ()) + (1,), at)
+    x, a, b, dz = view(ins, (N, K), 0), view(ins, (L, R, K), 100), view(ins, (L, R, U), 1000), view(ins, (N, U), 2000)
+    for t, v in ((x, xs), (a, as_), (b, bs), (dz, dzs)):
+        t.copy_(v)
+    out, da, db, dx = view(outs, (N, U), 0), view(outs, (L, R, K), 100), view(outs, (L, R, U), 1000), view(outs, (N, K), 2000)
+    want, _ = _formula(x, a, b, index, scale, dz)
+    # (the spans of interleaved outputs overlap, which the call refuses: each gets what it can be given)
+    _equal(ops.adapter_forward(x, a, b, index, scale, out=out), want['out'], 'out')
+    got = ops.adapter_backward(dz, x, a, b, index, scale, da=da)
+    _equal(da, want['da'], 'da'); _equal(got[1], want['db'], 'db')
+    got = ops.adapter_backward(dz, x, a, b, index, scale, db=db)
+    _equal(db, want['db'], 'db'); _equal(got[0], want['da'], 'da')
+    got = ops.adapter_backward(dz, x, a, b, index, scale, dx=dx)
+    _equal(dx, want['dx'], 'dx')
+
+
 def test_gradients_against_differences():
     """dL of L = sum(dz * out) along random whole-number directions: out is bilinear, so the difference quotient of a whole step is
     exact (the operator's own forward in whole numbers), and equals the gradient's inner product."""
@@ -248,10 +295,11 @@ def test_same_bits_every_time_and_apart_from_the_other_rows():
     assert torch.equal(out, first[0][perm])
 
 
-def test_on_a_side_stream_and_in_graphs():
+@pytest.mark.parametrize('N', [80, 700])
+def test_on_a_side_stream_and_in_graphs(N):
     """Two graphs captured one after the other, replayed in turn with eager work between, and calls on two streams at once:
     every result is the eager one."""
-    N, K, U, L, R = 80, 1000, 300, 5, 16
+    K, U, L, R = 1000, 300, 5, 16
     sets = [_inputs(N, K, U, L, R, torch.float32, s, whole=True) for s in (1, 2)]
     want = [(ops.adapter_forward(*s[:5]),) + ops.adapter_backward(s[5], *s[:5], want_dx=True) for s in sets]
     streams = [torch.cuda.Stream() for _ in sets]

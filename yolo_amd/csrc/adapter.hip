@@ -99,6 +99,7 @@ __device__ inline int tile_by_ballots(const Plan &p, int t, int TM, TileLds &lds
         if (in) lds.rows[slot] = 64 * w + lane;        // all waves write the same: each reads what it wrote itself
         count += __popcll(__ballot(in));
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     return count;
 }
@@ -539,8 +540,7 @@ __device__ inline f32x4 load4(const T *p, int left) {
     return v;
 }
 
-// dst[row][r] (row stride LD) = f * sum_s part[s][rows[row]][r]; also stored to keep (N, R), without f.  A row of part has ldp
-// values: R16 (a kernel's partial sums; repeats for r in [R, R16), taken as zeros) or R (the caller's h).
+// dst[row][r] (row stride LD) = f * sum_s part[s][rows[row]][r], zero for r in [R, R16); also stored to keep (N, R), without f
 __device__ inline void put4(float *dst, f32x4 v, float f, float *keep, long long n, int r, int R) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -550,23 +550,18 @@ __device__ inline void put4(float *dst, f32x4 v, float f, float *keep, long long
     }
 }
 template <int R16, int LD>
-__device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ part, int ldp, int slices, int N, const int *rows, int count, int R,
+__device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ part, int slices, int N, const int *rows, int count, int R,
                             float f, float *keep) {
     constexpr int R4 = R16 / 4;
     const int tid = threadIdx.x;
-    const long long slab = (long long)N * ldp;
-    if (ldp != R16) {
-        for (int e = tid; e < count * R16; e += 256) {
-            const int row = e / R16, r = e % R16;
-            dst[row * LD + r] = r < R ? f * part[(long long)rows[row] * ldp + r] : 0.f;
-        }
-    } else if (slices > 4 && N * R4 <= 64) {           // a batch of few values: 4 to 8 threads to a value, as many for every tile
+    const long long slab = (long long)N * R16;
+    if (slices > 4 && N * R4 <= 64) {           // a batch of few values: 4 to 8 threads to a value, as many for every tile
         const int n = N * R4, most = 256 / n, groups = most < 8 ? most : 8, e = tid % n, g = tid / n, row = e / R4, r = 4 * (e % R4);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (g < groups && row < count) {
-            const float *src = part + (long long)rows[row] * ldp + r;
+            const float *src = part + (long long)rows[row] * R16 + r;
 #pragma unroll 8
-            for (int s = g; s < slices; s += groups) v += *(const f32x4_m *)(src + s * slab);
+            for (int s = g; s < slices; s += groups) v += *(const f32x4 *)(src + s * slab);
         }
         lds[tid] = v;
         __syncthreads();
@@ -578,10 +573,10 @@ __device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ pa
     } else {
         for (int e = tid; e < count * R4; e += 256) {
             const int row = e / R4, r = 4 * (e % R4);
-            const float *src = part + (long long)rows[row] * ldp + r;
-            f32x4 v = *(const f32x4_m *)src;
+            const float *src = part + (long long)rows[row] * R16 + r;
+            f32x4 v = *(const f32x4 *)src;
 #pragma unroll 8
-            for (int s = 1; s < slices; ++s) v += *(const f32x4_m *)(src + s * slab);
+            for (int s = 1; s < slices; ++s) v += *(const f32x4 *)(src + s * slab);
             put4(dst + row * LD + r, v, f, keep, rows[row], r, R);
         }
     }
@@ -642,7 +637,7 @@ __global__ __launch_bounds__(256, RT <= 2 || NT * RT == 4 ? 3 : 1) void expand_k
     };
     load(m, u);
     for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
-    join<R16, LD>(h, sums, a.part, R16, a.slices, p.N, rows, count, a.R, a.scale[adapter], keep);
+    join<R16, LD>(h, sums, a.part, a.slices, p.N, rows, count, a.R, a.scale[adapter], keep);
     float *at[NT][4];
 #pragma unroll
     for (int b = 0; b < NT; ++b)
@@ -715,6 +710,7 @@ __device__ inline int rows_by_ballots(const Plan &p, int i, int *rows) {
         if (mine) rows[total + __popcll(vote & ((1ull << lane) - 1))] = n;
         total += __popcll(vote);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     return total;
 }
@@ -843,7 +839,8 @@ __global__ __launch_bounds__(256) void join_kernel(float *part, long long n4, in
 
 // ------------------------------------------------------------------------------------------------------------- the host
 int check_sizes(const char *what, int N, int K, int U, int L, int R) {
-    TY1_REQUIRE(N >= 0 && K > 0 && U > 0, "%s: bad dimensions N=%d K=%d U=%d", what, N, K, U);
+    constexpr int kMost = 1 << 30;
+    TY1_REQUIRE(N >= 0 && K > 0 && U > 0 && N <= kMost && K <= kMost && U <= kMost, "%s: bad dimensions N=%d K=%d U=%d", what, N, K, U);
     TY1_REQUIRE(L >= 1 && L <= kMaxAdapters, "%s: %d adapters, 1 to %d are supported", what, L, kMaxAdapters);
     TY1_REQUIRE(R >= 1 && R <= kMaxRank, "%s: rank %d, 1 to %d are supported", what, R, kMaxRank);
     return 0;

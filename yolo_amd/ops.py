@@ -536,8 +536,8 @@ def _adapter_operands(x, a, b, index, scale):
     L, R, U = b.shape
     if not (1 <= R <= MAX_RANK and 1 <= L <= MAX_ADAPTERS):
         raise ValueError(f'{L} adapters of rank {R}: 1 to {MAX_ADAPTERS} of rank 1 to {MAX_RANK} are supported')
-    if K < 1 or U < 1 or max(N, K, U) >= 2 ** 31:
-        raise ValueError(f'x (N,K) = {(N, K)}, b (L,R,U) = {(L, R, U)}: sizes must be positive (N may be 0) and below 2^31')
+    if K < 1 or U < 1 or max(N, K, U) > 2 ** 30:
+        raise ValueError(f'x (N,K) = {(N, K)}, b (L,R,U) = {(L, R, U)}: sizes must be positive (N may be 0) and at most 2^30')
     if (a.dtype is x.dtype and b.dtype is x.dtype and a.get_device() == dev and b.get_device() == dev and a.shape == (L, R, K)
             and index.dtype is torch.int32 and index.get_device() == dev and index.shape == (N,) and index.is_contiguous()
             and scale.dtype is torch.float32 and scale.get_device() == dev and scale.shape == (L,) and scale.is_contiguous()
