@@ -590,92 +590,100 @@ struct ExpandArgs {
     const float *scale;        // (L)
     float *out, *keep;         // (N, U) stride ldo; (N, R) or null
     long long ldm, sm, ldo;
-    int U, R, slices, spans, span, accumulate;     // a workgroup takes `span` blocks of 256 columns; `spans` of them cover U
-    int TM, subs;              // rows of a tile; a workgroup takes 16 NT of them, `subs` workgroups cover the tile
+    int U, R, slices, blocks, accumulate;          // `blocks` of 256 columns, one to a workgroup
+    int TM, subs, max_tiles;   // rows of a tile; a workgroup takes 16 NT of them, `subs` workgroups cover the tile
 };
 
 template <class T, int NT, int RT>
-__global__ __launch_bounds__(256, RT <= 2 || NT * RT == 4 ? 3 : 1) void expand_kernel(const ExpandArgs<T> a, const Plan p) {
-    constexpr int TM = 16 * NT, R16 = 16 * RT, LD = R16 + 4, STEPS = R16 / 4;
+__global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_kernel(const ExpandArgs<T> a, const Plan p) {
+    constexpr int TM = 16 * NT, R16 = 16 * RT, LD = R16 + 4;
     __shared__ TileLds tl;
     __shared__ __attribute__((aligned(16))) float h[TM * LD];
     __shared__ f32x4 sums[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-    const int whole = blockIdx.x / a.spans, first = (blockIdx.x - whole * a.spans) * a.span, t = whole / a.subs, sub = whole - t * a.subs;
+    // Workgroups that read the same part of m belong on one XCD (blockIdx % 8), whose L2 then fetches it once: the tiles of an
+    // adapter on the same columns where there are 8 column blocks or more, the row blocks of a tile below that (gradient of x
+    // at 2048 rows x 12544: 41 -> 38 us; 4096 rows x 539 of rank 64: 24 -> 22.5).
+    int t, sub, block;
+    if (a.blocks >= 8) {
+        const int b8 = (a.blocks + 7) & ~7, ts = blockIdx.x / b8;
+        block = blockIdx.x - ts * b8;
+        t = ts / a.subs;
+        sub = ts - t * a.subs;
+    } else {
+        const int g = blockIdx.x >> 3, gs = g / a.subs, pair = gs * 8 + (blockIdx.x & 7);
+        sub = g - gs * a.subs;
+        t = pair / a.blocks;
+        block = pair - t * a.blocks;
+    }
+    if (t >= a.max_tiles || block >= a.blocks) return;
     int adapter;
-    const int all = find_tile(p, t, a.TM, tl, adapter) - sub * TM, count = all < TM ? all : TM;
+    const int all = find_tile(p, t, a.TM, tl, adapter) - sub * TM, count = __builtin_amdgcn_readfirstlane(all < TM ? all : TM);
     if (count <= 0) return;
     const int *rows = tl.rows + sub * TM;
-    float *keep = first == 0 ? a.keep : nullptr;
-    const int u_end = (first + a.span) * 256 < a.U ? (first + a.span) * 256 : a.U;
+    float *keep = block == 0 ? a.keep : nullptr;
     if (adapter >= p.L) {                              // no adapter: zeros (or out as it is); an index behind the bank: NaN
+        const int c = block * 256 + tid;
         for (int row = 0; row < count; ++row) {
             const int n = rows[row];
             const bool bad = p.index[n] >= 0;
             const float v = bad ? __builtin_nanf("") : 0.f;
-            if (bad || !a.accumulate)
-                for (int c = first * 256 + tid; c < u_end; c += 256) a.out[n * a.ldo + c] = v;
+            if ((bad || !a.accumulate) && c < a.U) a.out[n * a.ldo + c] = v;
             if (keep && tid < a.R) keep[(long long)n * a.R + tid] = v;
         }
         return;
     }
-    f32x4 m[STEPS];                                    // step k of lane (j, q): rank q * STEPS + k, the same order as h's
-    int u = first * 256 + wave * 64 + 4 * j;
-    const T *mp = a.m + adapter * a.sm;
-    auto load = [&](f32x4 *v, int c) {
-        if (c - 4 * j + 64 <= a.U) {                   // (uniform) all of the wave's columns are there
+    const int u = block * 256 + wave * 64 + 4 * j, left = a.U - u;
+    const T *mp = a.m + adapter * a.sm + u;
+    auto load = [&](f32x4 (&v)[4], int r0) {           // ranks r0 + 4 q .. r0 + 4 q + 3 of this lane's columns
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) v[k] = load4(mp + (q * STEPS + k < a.R ? q * STEPS + k : 0) * a.ldm + c);
-        } else {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) v[k] = c < a.U ? load4(mp + (q * STEPS + k < a.R ? q * STEPS + k : 0) * a.ldm + c, a.U - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 4; ++e) {
+            const int r = r0 + 4 * q + e;
+            const T *at = mp + (r < a.R ? r : 0) * a.ldm;
+            if (u - 4 * j + 64 <= a.U) v[e] = load4(at);             // (uniform) all of the wave's columns are there
+            else v[e] = left > 0 ? load4(at, left) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (a.R < R16)                                 // ranks that are not there: zeros on both sides
+        if (r0 + 16 > a.R)                             // ranks that are not there: zeros on both sides
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-                if (q * STEPS + k >= a.R) v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; ++e)
+                if (r0 + 4 * q + e >= a.R) v[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
-    load(m, u);
+    // One row block: 16 ranks at a time, the next ones on their way (few registers, many workgroups to a CU).  Several: all ranks
+    // stay in registers for them.
+    constexpr int HELD = NT == 1 && RT > 1 ? 2 : RT;
+    f32x4 m[HELD][4];
+#pragma unroll
+    for (int k = 0; k < (NT == 1 ? 1 : RT); ++k) load(m[k], 16 * k);
     for (int e = tid; e < (TM - count) * LD; e += 256) h[count * LD + e] = 0.f;
     join<R16, LD>(h, sums, a.part, a.slices, p.N, rows, count, a.R, a.scale[adapter], keep);
-    float *at[NT][4];
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+    for (int b = 0; b < NT; ++b) {
+        if (16 * b >= count) break;
+        f32x4 acc[4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) at[b][v] = a.out + rows[16 * b + 4 * q + v < count ? 16 * b + 4 * q + v : 0] * a.ldo;
-    for (;;) {
-        const int left = a.U - u;
-        const bool more = u - 4 * j + 256 < u_end;
+        for (int c = 0; c < 4; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            if (16 * b >= count) break;
-            f32x4 acc[4];
+        for (int k = 0; k < RT; ++k) {
+            if (NT == 1 && k + 1 < RT) load(m[(k + 1) % HELD], 16 * (k + 1));
+            const f32x4 hv = *(const f32x4 *)(h + (16 * b + j) * LD + 16 * k + 4 * q);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int k = 0; k < STEPS; k += 4) {
-                const f32x4 hv = *(const f32x4 *)(h + (16 * b + j) * LD + q * STEPS + k);
+                for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[e], m[k % HELD][e][c], acc[c], 0, 0, 0);
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[e], m[k + e][c], acc[c], 0, 0, 0);
-            }
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                if (16 * b + 4 * q + v >= count || left <= 0) continue;
-                float *o = at[b][v] + u;
-                f32x4 val = {acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
-                if (left >= 4) {
-                    if (a.accumulate) val += load4(o);
-                    *(f32x4_m *)o = val;
-                } else {
-                    for (int e = 0; e < left; ++e) o[e] = a.accumulate ? o[e] + val[e] : val[e];
-                }
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * b + 4 * q + v;
+            if (row >= count || left <= 0) continue;
+            float *o = a.out + rows[row] * a.ldo + u;
+            f32x4 val = {acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
+            if (left >= 4) {
+                if (a.accumulate) val += load4(o);
+                *(f32x4_m *)o = val;
+            } else {
+                for (int e = 0; e < left; ++e) o[e] = a.accumulate ? o[e] + val[e] : val[e];
             }
         }
-        if (!more) break;
-        u += 256;
-        load(m, u);
     }
 }
 
@@ -935,14 +943,10 @@ void contract(const Layout &y, const Plan &p, const TX *x, long long ldx, const 
 template <class T>
 void expand(const Layout &y, const Plan &p, const float *part, int slices, const T *m, long long ldm, long long sm, const float *scale, float *out,
             long long ldo, float *keep, int U, int R, int accumulate, hipStream_t s) {
-    // Few workgroups: 16 rows each instead of the tile's height (4096 rows x 539 of rank 64: 29 us with 64 rows a workgroup).
-    // Plenty: several blocks of columns each, h is joined once for all of them.
+    // few workgroups: 16 rows each instead of the tile's height
     const int blocks = (U + 255) / 256, nt = (long long)y.max_tiles * blocks < 1024 ? 1 : y.nt, subs = y.nt / nt;
-    int span = (int)((long long)y.max_tiles * blocks / 1024);
-    span = span < 1 ? 1 : span > blocks ? blocks : span;
-    const int spans = (blocks + span - 1) / span;
-    const ExpandArgs<T> a = {part, m, scale, out, keep, ldm, sm, ldo, U, R, slices, spans, span, accumulate, 16 * y.nt, subs};
-    const dim3 grid((unsigned)(y.max_tiles * subs * spans));
+    const ExpandArgs<T> a = {part, m, scale, out, keep, ldm, sm, ldo, U, R, slices, blocks, accumulate, 16 * y.nt, subs, y.max_tiles};
+    const dim3 grid((unsigned)(blocks >= 8 ? y.max_tiles * subs * ((blocks + 7) & ~7) : (y.max_tiles * blocks + 7) / 8 * 8 * subs));
     Layout z = y;
     z.nt = nt;
 #define CALL(NT, RT) expand_kernel<T, NT, RT><<<grid, dim3(256), 0, s>>>(a, p)
@@ -983,7 +987,7 @@ int forward(const char *what, const T *x, const T *a, const T *b, const int32_t 
     const Layout y = layout(N, K, U, L, R, false);
     TY1_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y.bytes, "%s: workspace null, not 16-byte aligned, or %zu bytes where %zu are needed", what,
                 ws_bytes, y.bytes);
-    if (check_grid(what, y, y.slices) || check_grid(what, y, 4 * ((U + 255ll) / 256))) return 1;
+    if (check_grid(what, y, y.slices) || check_grid(what, y, 8 * ((U + 255ll) / 256))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_forward", s, 2.0 * N * R * ((double)K + U), sizeof(T) * ((double)N * K + (double)(L < N ? L : N) * R * ((double)K + U)) + 4.0 * N * U);
     const Plan p = make_plan(y, (char *)ws, index, N, L, s);
@@ -1012,7 +1016,7 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     const int wide = split ? 64 : 256;
     const long long ka = (K + wide - 1ll) / wide, ub = (U + wide - 1ll) / wide;
     TY1_REQUIRE(2 * L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
-    if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 4 * ((K + 255ll) / 256)))) return 1;
+    if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 8 * ((K + 255ll) / 256)))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_backward", s, 2.0 * N * R * (K * (dx ? 2.0 : 1.0) + 2.0 * U),
                         sizeof(T) * (double)N * K + 4.0 * N * U + 4.0 * L * R * ((double)K + U) + (dx ? 4.0 * N * K : 0.0));
