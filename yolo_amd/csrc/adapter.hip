@@ -8,7 +8,9 @@
 //
 // With A as [L][R][K] and B as [L][R][U] three kernels serve all of it: contract the long axis of a row against its adapter
 // (x.A^T and dz.B^T), expand the rank (h.B and g.A), and contract the rows of one adapter (g^T.x and h^T.dz).  All sums are
-// float32; bf16 operands are widened as they are read.
+// float32 on the matrix cores and nothing between x and out is rounded to less: bf16 operands multiply as they are (their products
+// are exact in float32) or are widened against float32 ones.  No atomics: every order of summation follows from the sizes, the
+// rows of an adapter are summed in ascending order, and a row's forward result does not depend on the rows beside it.
 #include "common.h"
 #include <type_traits>
 
@@ -208,12 +210,19 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
 
 // ------------------------------------------------------------------------------------------------------------- contract
 // part[s][n][r] = sum over K slice s of x[n][k] m[i][r][k], for the rows of one tile against their adapter: a GEMM tile of
-// TM rows x R ranks, K long.  Bound by reading x and m once.  A matrix fragment takes 16 bytes of each of 16 rows from
-// neighbouring lanes, which as a load from memory is 64 cache accesses an instruction (measured at 4096 rows of rank 64: the
-// cache's access rate held the kernel at 115 us); so a stage of 256 to 1024 consecutive bytes of every row goes through
-// registers into LDS, 16 accesses an instruction, and the fragments are read from there.  A row's 16-byte pieces are permuted
-// by its number: the 16 rows of a fragment read lie in 16 different bank groups.  The loads of the next stage are in flight
-// while the present one multiplies; every wave takes a quarter of a stage's K, and the four sums join in LDS.
+// TM rows x R ranks, K long.  Bound by reading x and m once.  Every wave takes a quarter of the slice, the four sums join in LDS.
+// Two forms:
+//   direct   Fragments come from memory straight into the registers of the matrix instruction: lane (j, q) of a 16-row fragment
+//            holds 16 consecutive bytes of row j at q * 16 bytes - four steps of v_mfma_f32_16x16x4_f32 with k in another
+//            order, the same on both sides, or one of v_mfma_f32_16x16x32_bf16.  No barrier before the end: the shortest way
+//            for one slice (one row x 12544 of rank 8: 4.5 us, most of it launch and three dependent loads; 64 rows of 16
+//            adapters of rank 16, 16 MB: 7.5 us).
+//   staged   A fragment load is 64 cache accesses an instruction (its neighbouring lanes are different rows), which is what
+//            bounds the direct form in the long run.  Here 256 consecutive bytes of every row go through registers into
+//            LDS, 16 accesses an instruction, and the fragments are read from there.  A row's 16-byte pieces are permuted by
+//            its number: the 16 rows of a fragment read lie in 16 different bank groups.  The loads of the next stage are in
+//            flight while the present one multiplies (a second LDS buffer and 512-byte stages measured slower).  4096 rows
+//            x 12544 of 64 adapters of rank 64 in float32: 104 us, 447 MB fetched = 4.3 TB/s, matrix pipe half busy.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) Piece_m {               // 16 bytes from wherever a row's elements lie
     u32x4 v;
@@ -238,8 +247,8 @@ struct ContractArgs {
     int K, R, slices;
 };
 
-// elements of K in a stage: 256 bytes a row for tall tiles, up to 1024 for low ones (two to ten loads a thread in flight)
-constexpr int stage_elements(int nt, int rt, int sx, int sw) { return (nt + rt <= 2 ? 1024 : nt + rt <= 3 || sx != sw ? 512 : 256) / sx; }
+// elements of K in a stage: 256 bytes a row of m (and so 512 of x where x is float32 and m bf16)
+constexpr int stage_elements(int sw) { return 256 / sw; }
 
 // The waves' sums of a tile, (0 + 2) + (1 + 3): into red[0 .. TM R16) + red[TM R16 ..).
 template <int NB, int NT, int RT>
@@ -267,7 +276,7 @@ __device__ inline void join_waves(const f32x4 (&acc)[NB][RT], float *red) {
     __syncthreads();
 }
 
-// The direct form.  (a) fragments of a lane:
+// The direct form: the fragments of a lane.
 template <class TX, class TW>
 struct Frag;
 template <>
@@ -304,7 +313,7 @@ __device__ inline V load_lane(const T *p, int left) {               // the first
     return v;
 }
 
-// (b) The waves take neighbouring groups of UN fragments in turn, so that the workgroup reads 256 consecutive bytes of a row or
+// The waves take neighbouring groups of UN fragments in turn, so that the workgroup reads 256 consecutive bytes of a row or
 // more at a time.  UN is the same for full and partial tiles: a row's sum does not depend on the tile it is in.
 template <class TX, class TW, int NB, int NT, int RT>
 __device__ inline void contract_direct(const ContractArgs<TX, TW> &a, const int *rows, int count, int adapter, int s, float *red) {
@@ -390,7 +399,7 @@ __device__ inline void contract_direct(const ContractArgs<TX, TW> &a, const int 
 template <class T, int ROWS, int KS>
 struct Carrier {
     static constexpr int E = 16 / sizeof(T), PPR = KS / E, LOADS = ROWS * PPR / 256, STEP = 256 / PPR;
-    static_assert(ROWS * PPR % 256 == 0 && PPR <= 256 && 256 % PPR == 0, "a stage is whole loads");
+    static_assert(ROWS * PPR % 256 == 0 && PPR >= 16 && 256 % PPR == 0, "a stage is whole loads");
     const T *src[LOADS];
     u32x4 reg[LOADS];
     // row(i) -> pointer to the row's first element of this slice
@@ -415,19 +424,19 @@ struct Carrier {
     __device__ void store(u32x4 *lds) const {
         const int piece = threadIdx.x % PPR, first = threadIdx.x / PPR;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) lds[(first + i * STEP) * PPR + (piece ^ ((first + i * STEP) & (PPR < 16 ? PPR - 1 : 15)))] = reg[i];
+        for (int i = 0; i < LOADS; ++i) lds[(first + i * STEP) * PPR + (piece ^ ((first + i * STEP) & 15))] = reg[i];
     }
 };
 
 template <class T, int KS>
 __device__ inline u32x4 fragment(const u32x4 *lds, int row, int piece) {
     constexpr int PPR = KS * sizeof(T) / 16;
-    return lds[row * PPR + (piece ^ (row & (PPR < 16 ? PPR - 1 : 15)))];
+    return lds[row * PPR + (piece ^ (row & 15))];
 }
 
 template <class TX, class TW, int NB, int NT, int RT>
 __device__ inline void contract_staged(const ContractArgs<TX, TW> &a, const int *rows, int count, int adapter, int s, u32x4 *lds) {
-    constexpr int R16 = 16 * RT, KS = stage_elements(NT, RT, sizeof(TX), sizeof(TW)), E = 16 / sizeof(TX), KC = 4 * E;
+    constexpr int R16 = 16 * RT, KS = stage_elements(sizeof(TW)), E = 16 / sizeof(TX), KC = 4 * E;
     constexpr int FRAGMENTS = KS / KC / 4;             // of a stage, for each wave
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
     const int chunks = (a.K + KC - 1) / KC;            // slices are cut between fragments
@@ -497,7 +506,7 @@ __device__ inline void contract_staged(const ContractArgs<TX, TW> &a, const int 
 
 template <class TX, class TW, int NT, int RT, bool STAGED>
 __global__ __launch_bounds__(256, 2) void contract_kernel(const ContractArgs<TX, TW> a, const Plan p) {
-    constexpr int TM = 16 * NT, R16 = 16 * RT, KS = stage_elements(NT, RT, sizeof(TX), sizeof(TW));
+    constexpr int TM = 16 * NT, R16 = 16 * RT, KS = stage_elements(sizeof(TW));
     constexpr int STAGE = STAGED ? (TM * sizeof(TX) + R16 * sizeof(TW)) * KS : 0, SUMS = 2 * TM * R16 * 4, BYTES = STAGE > SUMS ? STAGE : SUMS;
     __shared__ TileLds tl;
     __shared__ u32x4 lds[BYTES / 16];
@@ -525,7 +534,8 @@ __global__ __launch_bounds__(256, 2) void contract_kernel(const ContractArgs<TX,
 // out[n][u] (+)= sum_r h[n][r] m[i][r][u] with h = scale[i] sum_s part[s]: one wave per 64 columns, lane (j, q) holding four
 // consecutive ones, so that loads of m and stores of out are 256 bytes a row.  Bound by reading m and writing out.  h is
 // joined from the K slices on the way (and stored, without the scale, where the caller keeps it).  float32 matrix instruction
-// for both types: bf16 weights are widened, h is not rounded.
+// for both types: bf16 weights are widened, h is not rounded.  One row x 1470: 5.4 us; 4096 rows x 539 of rank 64: 20 us; the
+// gradient of x of 2048 rows x 12544 of rank 32: 39 us, 167 MB moved = 4.3 TB/s.
 __device__ inline f32x4 load4(const float *p) { return *(const f32x4_m *)p; }
 __device__ inline f32x4 load4(const bf16 *p) {
     const bf16x4_m v = *(const bf16x4_m *)p;
@@ -603,7 +613,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_ker
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
     // Workgroups that read the same part of m belong on one XCD (blockIdx % 8), whose L2 then fetches it once: the tiles of an
     // adapter on the same columns where there are 8 column blocks or more, the row blocks of a tile below that (gradient of x
-    // at 2048 rows x 12544: 41 -> 38 us; 4096 rows x 539 of rank 64: 24 -> 22.5).
+    // at 2048 rows x 12544: 39 -> 38 us; 4096 rows x 539 of rank 64: 24 -> 22.5).
     int t, sub, block;
     if (a.blocks >= 8) {
         const int b8 = (a.blocks + 7) & ~7, ts = blockIdx.x / b8;
@@ -691,8 +701,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_ker
 // out[i][r][k] = scale[i] sum over the rows n of adapter i of g[n][r] x[n][k], g = sum_s part[s]: lane (j, q) of a wave holds
 // four consecutive columns of row 4 step + q, so that loads of x and stores of out are 256 bytes a row.  Bound by reading x
 // and writing out once.  A wave runs through the adapter's rows by itself, 16 at a time, reading g from L2: a version that put
-// g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of rank 32: 81 us).  Two such products (A's
-// gradient and B's) share a launch.
+// g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of 16 adapters of rank 32: 81 us, now 43 to 54).
+// Two such products (A's gradient and B's) share a launch.  Loading the next 16 rows ahead costs more registers than it hides
+// latency (74 us): occupancy carries it.
 //   few rows to an adapter: a wave has 64 columns and all rows, a workgroup 256 columns;
 //   many (SPLIT): the four waves have the same 64 columns and a quarter of the rows each, joined in LDS (128 or 256 columns to
 //   a wave read g less often and measured slower, 54 against 61 and 99 us: the adapter with the most rows has too few waves).
@@ -874,9 +885,15 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     Layout y;
     y.rt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
     const int classes = L < N ? L : N;
-    y.nt = N >= 48ll * classes ? (y.rt == 8 ? 2 : 4) : 1;
-    const long long tiles = (long long)N / (16 * y.nt) + (L + 1 < N ? L + 1 : N);
-    y.max_tiles = (int)(tiles < N ? tiles : N > 1 ? N : 1);
+    // 64 rows to a tile (32 at ranks above 64) from 48 rows an adapter on, from 20 where the tiles and slices of 512 elements
+    // still make two workgroups a CU, and 16 rows below.  Forward, x 12544: 1024 rows of 32 adapters of rank 32 38 us tall, 50
+    // low; 4096 of 64 of rank 64 146 and 222; 1024 of 128 adapters of rank 16 45 tall, 42 low; 333 rows x 4999 of 7 adapters of
+    // rank 11 19 tall, 17 low.
+    const auto tiles = [&](int nt) { return (long long)N / (16 * nt) + (L + 1 < N ? L + 1 : N); };
+    const int tall = y.rt == 8 ? 2 : 4, axis = back ? U : K;
+    y.nt = N >= 48ll * classes || (N >= 20ll * classes && tiles(tall) * ((axis + 511) / 512) >= 512) ? tall : 1;
+    const long long most = tiles(y.nt);
+    y.max_tiles = (int)(most < N ? most : N > 1 ? N : 1);
     y.sorted = N > kSelfPlan;
     // Slices that every reader joins by itself: 512 elements (256 make one frame's contraction 0.7 us faster and what reads it
     // 1 us slower).  Joined by a launch of their own: 256 (2048 rows x 1470 of rank 32: 12.5 -> 10.2 us).
@@ -929,7 +946,7 @@ void contract(const Layout &y, const Plan &p, const TX *x, long long ldx, const 
     const ContractArgs<TX, TM> a = {x, m, part, ldx, ldm, sm, K, R, slices};
     const dim3 grid((unsigned)(y.max_tiles * slices));
     // staged where tall tiles fill the chip with long slices: 4096 rows x 12544 of rank 64 take 104 us against 115 to 130 direct;
-    // direct where latency counts: one row 4.7 us against 5.5, 2048 rows x 1470 of rank 32 13.0 against 15.9
+    // direct where latency counts: one row 4.7 us against 5.5, 2048 rows x 1470 of rank 32 in three slices 13.0 against 15.9
     const bool staged = y.nt > 1 && y.max_tiles * slices >= 512 && K / slices * (int)sizeof(TX) >= 2048;
 #define CALL(NT, RT)                                                                                 \
     do {                                                                                             \
@@ -1011,8 +1028,10 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     Layout y = layout(N, K, U, L, R, true);
     TY1_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y.bytes, "%s: workspace null, not 16-byte aligned, or %zu bytes where %zu are needed", what,
                 ws_bytes, y.bytes);
-    // many rows to an adapter: they are split over the waves of a workgroup (rows_tile)
-    const bool split = N > 32ll * (L < N ? L : N);
+    // Many rows to an adapter are split over the waves of a workgroup (rows_tile), unless the adapters fill the chip without it:
+    // 500 rows of 8 adapters at rank 16 12 us split, 31 not; 2048 of 16 at rank 32 54 and 142; 4096 of 64 at rank 64 (the whole
+    // call) 224 split, 174 not; 600 rows of 20 adapters, fewer than 32 each, 37 split, 33 not.
+    const bool split = N > 32ll * (L < N ? L : N) && L * ((K + 255ll) / 256 + (U + 255ll) / 256) < 2048;
     const int wide = split ? 64 : 256;
     const long long ka = (K + wide - 1ll) / wide, ub = (U + wide - 1ll) / wide;
     TY1_REQUIRE(2 * L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
