@@ -61,6 +61,31 @@ def test_a_batch_of_mixed_adapters(dtype):
     assert torch.equal(model.predict(x, bank, index), plain)
 
 
+def test_a_captured_detection_follows_the_bank():
+    """detect() with adapters as one graph: same bits, and new weights and another index take effect at the next replay."""
+    for dtype in ('f32', 'bf16'):
+        _, model, x, bank, which = _setup(dtype)
+        index = bank.index(which)
+        other = bank.index([2, 2, -1, 0, 1, 0])
+        want = [[t.clone() for t in model.detect(x, adapters=bank, index=i)] for i in (index, other)]
+        live = index.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = model.detect(x, adapters=bank, index=live)
+        for rep in range(4):
+            live.copy_((index, other)[rep % 2])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, want[rep % 2])), (dtype, rep)
+        bank.b.zero_()
+        bank.changed()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(p, q) for p, q in zip(got, model.detect(x)))
+
+
 def test_one_image_and_refusals():
     _, model, x, bank, _ = _setup()
     one = model.predict(x[:1], bank, bank.index([2])).clone()

@@ -345,6 +345,11 @@ def test_refusals():
             fwd(**kw)
         with pytest.raises(ValueError):
             bwd(**kw)
+    for name in ('a', 'b', 'index', 'scale'):
+        with pytest.raises(TypeError, match=name):
+            fwd(**{name: None})
+    with pytest.raises(TypeError, match='h'):
+        fwd(h=torch.zeros((N, R)))
     with pytest.raises(ValueError, match='rank'):
         ops.adapter_forward(x, torch.zeros((1, 129, K), device=DEV), torch.zeros((1, 129, U), device=DEV), index, scale[:1])
     for kw in (dict(accumulate=True), dict(out=torch.zeros((N, U + 1), device=DEV)), dict(h=torch.zeros((N, R + 1), device=DEV)), dict(h=torch.zeros((R, N), device=DEV).t()),

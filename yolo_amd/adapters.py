@@ -15,7 +15,7 @@ class AdapterBank:
     views of one flat float32 buffer (`flat`, what an optimiser updates in one launch; b's rows are padded to 16 bytes), and
     scale (count).  a starts uniform in +-1/sqrt(features), b at zero: a new adapter changes nothing.  Give a bank and one index
     per image (bank.index(...)) to DeviceModel.predict / detect / head, or train it with engine.AdapterTrainer.  For a bf16
-    model the products read bf16 copies; call changed() after writing to a or b yourself."""
+    model the products read a bf16 copy: call changed() after writing to a or b yourself."""
 
     def __init__(self, model, count, rank, scale=1.0, seed=1):
         count, rank = int(count), int(rank)
@@ -28,7 +28,8 @@ class AdapterBank:
         gen = torch.Generator().manual_seed(seed)
         self.a.copy_((torch.rand((count, rank, self.features), generator=gen) * 2 - 1) * self.features ** -0.5)
         self.scale = torch.full((count,), float(scale), dtype=torch.float32, device=self.device)
-        self._bf16 = None
+        self._bf16 = torch.zeros_like(self.flat, dtype=torch.bfloat16) if getattr(model, 'dtype', 'f32') == 'bf16' else None
+        self.changed()
 
     def views(self, flat):
         """a- and b-shaped views of a flat buffer of this bank's size (its gradients, its moments)."""
@@ -38,16 +39,19 @@ class AdapterBank:
             self.count, self.rank, ops.round_up(self.units, 4))[:, :, :self.units]
 
     def changed(self):
-        """a or b were written to: bf16 copies are made anew by the next product that reads them."""
-        self._bf16 = None
+        """a or b were written to: bring the bf16 copy of a bf16 model's bank up to date, in place, and wait for it (any stream may
+        read it next, and graphs that were captured with it read the new values)."""
+        if self._bf16 is not None:
+            ops.cast_bf16(self.flat, out=self._bf16)
+            torch.cuda.current_stream(self.device).synchronize()
 
     def weights(self, dtype):
-        """(a, b) for products in torch.float32 or torch.bfloat16."""
+        """(a, b) for products in torch.float32 or, in a bf16 model's bank, torch.bfloat16."""
         if dtype == torch.float32:
             return self.a, self.b
         if self._bf16 is None:
-            self._bf16 = self.views(ops.cast_bf16(self.flat))
-        return self._bf16
+            raise ValueError('the bank was made for a float32 model')
+        return self.views(self._bf16)
 
     def index(self, which):
         """Adapter numbers on the host, one per image (-1 or None: the shared weights alone) -> checked int32 tensor on the GPU."""

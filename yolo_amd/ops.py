@@ -501,6 +501,14 @@ def _strided(t, dtype, shape, index, name):
     return t
 
 
+def _dense_on(t, shape, index, name):
+    """A contiguous float32 tensor of this shape on device `index`."""
+    _strided(t, torch.float32, shape, index, name)
+    if not t.is_contiguous():
+        raise ValueError(f'{name}: must be contiguous')
+    return t
+
+
 def _span(t):
     """First and last address + 1 of a tensor's values."""
     lo = t.data_ptr()
@@ -529,6 +537,9 @@ def _adapter_operands(x, a, b, index, scale):
         raise TypeError('x: expected a tensor on the GPU (ROCm device)')
     if x.dtype is not torch.float32 and x.dtype is not torch.bfloat16:
         raise TypeError(f'x: expected torch.float32 or torch.bfloat16, got {x.dtype}')
+    for name, t in (('a', a), ('b', b), ('index', index), ('scale', scale)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'{name}: expected a tensor on the GPU, got {type(t).__name__}')
     if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError(f'expected x (N,K), a (L,R,K), b (L,R,U), got {tuple(x.shape)}, {tuple(a.shape)}, {tuple(b.shape)}')
     dev = x.get_device()
@@ -564,11 +575,11 @@ def adapter_forward(x, a, b, index, scale, out=None, accumulate=False, h=None):
             raise ValueError('accumulate needs out')
         out = torch.empty((N, U), dtype=torch.float32, device=x.device)
         if h is not None:
-            _chk_written([('h', _chk_out(h, torch.float32, (N, R), 'h'))], [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
+            _chk_written([('h', _dense_on(h, (N, R), dev, 'h'))], [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
     else:
         outs = [('out', _strided(out, torch.float32, (N, U), dev, 'out'))]
         if h is not None:
-            outs.append(('h', _chk_out(h, torch.float32, (N, R), 'h')))
+            outs.append(('h', _dense_on(h, (N, R), dev, 'h')))
         _chk_written(outs, [('x', x), ('a', a), ('b', b), ('index', index), ('scale', scale)])
     if N == 0:
         return out
@@ -588,9 +599,7 @@ def adapter_backward(dz, x, a, b, index, scale, h=None, want_dx=False, da=None, 
     dev, N, K, U, L, R = _adapter_operands(x, a, b, index, scale)
     _strided(dz, torch.float32, (N, U), dev, 'dz')
     if h is not None:
-        _strided(h, torch.float32, (N, R), dev, 'h')
-        if not h.is_contiguous():
-            raise ValueError('h: must be contiguous')
+        _dense_on(h, (N, R), dev, 'h')
     if da is not None or db is not None or dx is not None:
         given = [(name, _strided(t, torch.float32, shape, dev, name)) for name, t, shape in
                  (('da', da, (L, R, K)), ('db', db, (L, R, U)), ('dx', dx, (N, K))) if t is not None]
@@ -660,7 +669,7 @@ def _norm_workspace_bytes(n):
 def _norm_buffers(dev, n, norm):
     device = torch.device('cuda', dev)
     ws = torch.empty((_norm_workspace_bytes(n),), dtype=torch.uint8, device=device)
-    return ws, torch.empty((1,), dtype=torch.float32, device=device) if norm is None else _chk_out(norm, torch.float32, (1,), 'norm')
+    return ws, torch.empty((1,), dtype=torch.float32, device=device) if norm is None else _dense_on(norm, (1,), dev, 'norm')
 
 
 def _max_norm(v):
