@@ -282,7 +282,8 @@ int ty1_adam_step_f32(float *p, const float *g, float *m, float *v, int64_t n, f
  * x (N,K); a (L,R,K); b (L,R,U): element (i,r,c) of a at a + i*sa + r*lda + c, of b at b + i*sb + r*ldb + c, row n of x at
  * x + n*ldx (strides in elements; the last axis is dense).  _f32: x, a, b float32.  _bf16: x, a, b bf16.  index (N) int32,
  * scale (L) f32, out (N,U) f32 with row stride ldo, h (N,R) f32 or NULL: kept for the backward pass (without scale).  All
- * sums are float32.  1 <= R <= 128, 1 <= L <= 4096, any N, K, U; a smaller rank is padded with zero rows of A and B.
+ * sums are float32.  1 <= R <= 128, 1 <= L <= 4096, N, K, U up to 2^30; a smaller rank is padded with zero rows of A and B.
+ * out and h must not overlap the operands or one another (nor da, db, dx below).
  * workspace: scratch of ty1_adapter_workspace_bytes() bytes, 16-byte aligned, for this call alone.  Laid out as one more split of ty1_dense_splitk_f32's partials, out is summed by whatever kernel reduces those.
  */
 int ty1_adapter_workspace_bytes(int N, int K, int U, int L, int R, int backward, size_t *bytes);
@@ -302,7 +303,7 @@ int ty1_adapter_forward_bf16(const void *x, const void *a, const void *b, const 
  *   dx[n][k]    = sum_r g[n][r] A[i][r][k]                        (dx NULL: not computed)
  * da (L,R,K), db (L,R,U), dx (N,K) are f32 and written whole: an adapter without rows gets zeros, a row without an adapter a
  * zero dx row, a row with index >= L a NaN dx row and no part in da and db.  h as ty1_adapter_forward_* stored it, or NULL:
- * computed again.  Rows of an adapter are summed in ascending order of n: the same bits every time.
+ * computed again.  The rows of an adapter are summed in a fixed order: the same bits every time.
  */
 int ty1_adapter_backward_f32(const float *dz, const float *x, const float *a, const float *b, const int32_t *index,
                              const float *scale, const float *h, float *da, float *db, float *dx, int N, int K, int U, int L,

@@ -9,8 +9,8 @@
 // With A as [L][R][K] and B as [L][R][U] three kernels serve all of it: contract the long axis of a row against its adapter
 // (x.A^T and dz.B^T), expand the rank (h.B and g.A), and contract the rows of one adapter (g^T.x and h^T.dz).  All sums are
 // float32 on the matrix cores and nothing between x and out is rounded to less: bf16 operands multiply as they are (their products
-// are exact in float32) or are widened against float32 ones.  No atomics: every order of summation follows from the sizes, the
-// rows of an adapter are summed in ascending order, and a row's forward result does not depend on the rows beside it.
+// are exact in float32) or are widened against float32 ones.  No atomics: every order of summation follows from the sizes and from
+// which rows an adapter has, and a row's own results (out, h, dx) do not depend on the rows beside it in a batch of that size.
 #include "common.h"
 #include <type_traits>
 
@@ -565,7 +565,7 @@ __device__ inline void join(float *dst, f32x4 *lds, const float *__restrict__ pa
     constexpr int R4 = R16 / 4;
     const int tid = threadIdx.x;
     const long long slab = (long long)N * R16;
-    if (slices > 4 && N * R4 <= 64) {           // a batch of few values: 4 to 8 threads to a value, as many for every tile
+    if (slices > 4 && N <= 64 / R4) {           // a batch of few values: 4 to 8 threads to a value, as many for every tile
         const int n = N * R4, most = 256 / n, groups = most < 8 ? most : 8, e = tid % n, g = tid / n, row = e / R4, r = 4 * (e % R4);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (g < groups && row < count) {
