@@ -117,7 +117,20 @@ LONG = [(4000, 9001, 33, 2, 64, torch.float32), (2100, 9003, 20, 1, 100, torch.f
         (4000, 9001, 35, 3, 9, torch.float32), (4000, 16500, 20, 2, 40, torch.bfloat16), (4000, 40, 9001, 2, 30, torch.bfloat16),
         (4000, 40, 9001, 2, 61, torch.bfloat16), (2100, 30, 9002, 1, 128, torch.bfloat16), (4000, 64, 4100, 2, 17, torch.float32),
         (40, 100, 50, 5, 100, torch.float32), (600, 20, 16, 4096, 3, torch.float32), (256, 40, 20, 4096, 2, torch.bfloat16),
-        (257, 513, 1025, 1, 1, torch.float32)]
+        (257, 513, 1025, 1, 1, torch.float32), (2049, 303, 77, 700, 5, torch.float32), (5000, 130, 61, 1500, 18, torch.bfloat16)]
+
+
+def test_one_adapter_with_most_of_the_rows():
+    """Adapters of 0, 1, 256, 257, 512, 513 and the rest of 4000 rows: one piece, several, whole last ones and single rows."""
+    N, K, U, L, R = 4000, 301, 70, 8, 12
+    x, a, b, _, scale, dz = _inputs(N, K, U, L, R, torch.float32, 12, whole=True)
+    counts = [0, 1, 256, 257, 512, 513, N - 1 - 256 - 257 - 512 - 513 - 40]
+    index = torch.cat([torch.full((c,), i) for i, c in enumerate(counts)] + [torch.full((40,), -1)])
+    index = index[torch.randperm(N, generator=torch.Generator().manual_seed(2))].to(torch.int32).to(DEV)
+    want, mag = _formula(x, a, b, index, scale, dz)
+    assert max(float(m.max()) for m in mag.values()) < 2 ** 22
+    da, db, dx = ops.adapter_backward(dz, x, a, b, index, scale, want_dx=True)
+    _equal(da, want['da'], 'da'); _equal(db, want['db'], 'db'); _equal(dx, want['dx'], 'dx')
 
 
 @pytest.mark.parametrize('N, K, U, L, R, dtype', LONG)
@@ -281,10 +294,11 @@ def test_nothing_to_do():
     assert int(da.count_nonzero()) == 0 and int(db.count_nonzero()) == 0 and dx.shape == (0, 20)
 
 
-def test_same_bits_every_time_and_apart_from_the_other_rows():
+@pytest.mark.parametrize('N', [500, 2500])
+def test_same_bits_every_time_and_apart_from_the_other_rows(N):
     """A run repeated gives the same bits; so does a row's result whatever rows stand beside it in the batch, as long as the
     batch takes the same variant (same N)."""
-    N, K, U, L, R = 500, 3000, 200, 6, 16
+    K, U, L, R = 3000, 200, 6, 16
     x, a, b, index, scale, dz = _inputs(N, K, U, L, R, torch.float32, 77, whole=False)
     first = (ops.adapter_forward(x, a, b, index, scale),) + ops.adapter_backward(dz, x, a, b, index, scale, want_dx=True)
     for _ in range(3):

@@ -28,6 +28,7 @@ typedef __bf16 bf16x4_m __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int kMaxRank = 128, kMaxAdapters = 4096;
 constexpr int kSelfPlan = 256;            // rows up to which every workgroup finds its tile by itself
+constexpr int kPiece = 256;               // rows of an adapter that one workgroup sums for its gradient in a long batch
 
 // ---------------------------------------------------------------------------------------------------------------- tiles
 // The rows of a batch come in any order of adapters; a tile is up to TM rows of ONE adapter, so that the adapter's weights are
@@ -40,6 +41,7 @@ struct Plan {
     const int *perm;           // (N) rows, stably sorted by class        | null: N <= kSelfPlan
     const int *offs;           // (L + 1) first place of each class in perm
     const int4 *tiles;         // {class, first place, rows, -}, the unused ones without rows
+    const int4 *pieces;        // backward of long batches: {adapter or -1, first place, up to kPiece rows, slot or -1}  | null
 };
 
 __device__ inline int class_of(int i, int L) { return i < 0 || i >= L ? L : i; }
@@ -122,12 +124,15 @@ __device__ inline int find_tile(const Plan &p, int t, int TM, TileLds &lds, int 
 }
 
 // One workgroup sorts the rows by class (a stable counting sort, so that an adapter's rows stay in ascending order) and cuts
-// the classes into tiles.  Each wave owns a contiguous segment of the rows: counts them by class in LDS, the counts turn into
+// the classes into tiles and, where pieces are asked for, the adapters into pieces of up to kPiece rows: an adapter with more than
+// one piece gets a slot for each (what its pieces sum waits there to be joined).  Each wave owns a contiguous segment of the rows: counts them by class in LDS, the counts turn into
 // first places (class by class, segment by segment), and each wave puts its rows down in order, equal classes within 64 rows
 // ranked by ballots over the bits of the class.
+template <bool PIECES>
 __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ index, int N, int L, int waves, int bits, int TM,
                                                     int *__restrict__ perm, int *__restrict__ offs, int4 *__restrict__ tiles,
-                                                    int max_tiles) {
+                                                    int max_tiles, int4 *__restrict__ pieces, int max_pieces, int2 *__restrict__ slots,
+                                                    int max_slots) {
     extern __shared__ int hist[];                     // [waves][L + 1]
     __shared__ long long scan[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, C = L + 1;
@@ -149,29 +154,43 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
         for (long long n = lo + 64 * KEEP + lane; n < hi; n += 64) atomicAdd(&hist[wave * C + class_of(index[n], L)], 1);
     }
     __syncthreads();
-    long long carry = 0;                              // rows in the low half, tiles in the high half
-    for (int c0 = 0; c0 < C; c0 += 1024) {
-        const int c = c0 + tid;
-        int rows = 0;
-        if (c < C)
-            for (int w = 0; w < waves; ++w) rows += hist[w * C + c];
-        long long v = (long long)((rows + TM - 1) / TM) << 32 | rows;
+    // what comes before this thread's two counts (low and high half), over all threads and the classes before them
+    auto before_me = [&](long long v, long long &carry) {
         const long long mine = v;
         for (int d = 1; d < 64; d <<= 1) {
             const long long o = __shfl_up(v, d, 64);
             if (lane >= d) v += o;
         }
+        __syncthreads();
         if (lane == 63) scan[wave] = v;
         __syncthreads();
-        long long before = carry + v - mine, all = 0;
+        long long before = carry + v - mine;
+#pragma unroll 4
         for (int w = 0; w < 16; ++w) {
             if (w < wave) before += scan[w];
-            all += scan[w];
+            carry += scan[w];
         }
-        carry += all;
+        return before;
+    };
+    long long carry = 0, carry2 = 0;                  // tiles and rows; slots and pieces
+    for (int c0 = 0; c0 < C; c0 += 1024) {
+        const int c = c0 + tid;
+        int rows = 0;
+        if (c < C)
+            for (int w = 0; w < waves; ++w) rows += hist[w * C + c];
+        const long long before = before_me((long long)((rows + TM - 1) / TM) << 32 | rows, carry);
+        const int first = (int)(before & 0xffffffff);
+        if (PIECES) {
+            const int n = c >= L ? 0 : rows > kPiece ? (rows + kPiece - 1) / kPiece : 1, kept_apart = n > 1 ? n : 0;
+            const long long b2 = before_me((long long)kept_apart << 32 | n, carry2);
+            const int at = (int)(b2 & 0xffffffff), slot = (int)(b2 >> 32);
+#pragma unroll 1
+            for (int i = 0; i < n; ++i) pieces[at + i] = make_int4(c, first + i * kPiece, rows - i * kPiece < kPiece ? rows - i * kPiece : kPiece, n > 1 ? slot + i : -1);
+#pragma unroll 1
+            for (int i = 0; i < kept_apart; ++i) slots[slot + i] = make_int2(c, i == 0 ? n : 0);
+        }
         if (c < C) {
-            int place = (int)(before & 0xffffffff);
-            int t = (int)(before >> 32);
+            int place = first, t = (int)(before >> 32);
             offs[c] = place;
             for (int at = 0; at < rows; at += TM) tiles[t++] = make_int4(c, place + at, rows - at < TM ? rows - at : TM, 0);
             for (int w = 0; w < waves; ++w) {
@@ -182,11 +201,16 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
         }
         __syncthreads();
     }
+    if (PIECES) {
+        for (int t = (int)(carry2 & 0xffffffff) + tid; t < max_pieces; t += 1024) pieces[t] = make_int4(-1, 0, 0, -1);
+        for (int t = (int)(carry2 >> 32) + tid; t < max_slots; t += 1024) slots[t] = make_int2(0, 0);
+    }
     for (int t = (int)(carry >> 32) + tid; t < max_tiles; t += 1024) tiles[t] = make_int4(0, 0, 0, 0);
     if (wave < waves) {
         volatile int *mine = hist + wave * C;
         auto put = [&](int cls, long long n) {
             unsigned long long same = __ballot(cls >= 0);
+#pragma unroll 1
             for (int b = 0; b < bits; ++b) {
                 const unsigned long long set = __ballot(cls >> b & 1);
                 same &= cls >> b & 1 ? set : ~set;
@@ -704,7 +728,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_ker
 // g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of 16 adapters of rank 32: 81 us, now 43 to 54).
 // Two such products (A's gradient and B's) share a launch.  Loading the next 16 rows ahead costs more registers than it hides
 // latency (74 us): occupancy carries it.
-//   few rows to an adapter: a wave has 64 columns and all rows, a workgroup 256 columns;
+//   few rows to an adapter: a wave has 64 columns and all rows of the adapter or piece, a workgroup 256 columns;
 //   many (SPLIT): the four waves have the same 64 columns and a quarter of the rows each, joined in LDS (128 or 256 columns to
 //   a wave read g less often and measured slower, 54 against 61 and 99 us: the adapter with the most rows has too few waves).
 template <class T>
@@ -713,7 +737,9 @@ struct RowsArgs {
     const T *x;                // (N, K) stride ldx
     float *out;                // (L, R, K) strides so, ldo
     long long ldx, ldo, so;
-    int K, slices, ldp, blocks, ranks;     // `blocks` workgroups to an adapter and 64 ranks, `ranks` times 64 ranks
+    int K, slices, ldp, blocks, ranks;     // `blocks` workgroups to an adapter (or piece) and 64 ranks, `ranks` times 64 ranks
+    float *apart;              // (slots, R, lda) sums of the pieces of adapters with several
+    long long lda;             // K rounded up to 16 bytes
 };
 
 // the rows of adapter i in ascending order, up to kSelfPlan of them: every wave writes and reads the same list
@@ -737,11 +763,18 @@ __device__ inline int rows_by_ballots(const Plan &p, int i, int *rows) {
 template <class T, int RT, bool SPLIT>
 __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const float *scale, int R, int block, float *red, int *own) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
-    const int ir = block / a.blocks, cb = block - ir * a.blocks, i = ir / a.ranks, r0 = 64 * (ir - i * a.ranks);
+    const int ir = block / a.blocks, cb = block - ir * a.blocks, item = ir / a.ranks, r0 = 64 * (ir - item * a.ranks);
     const int k0 = SPLIT ? cb * 64 : cb * 256 + wave * 64, k = k0 + 4 * j;
-    int total;
+    int total, i = item, slot = -1;
     const int *rows = own;                             // (LDS) or the sorted list's
-    if (p.perm) {
+    if (p.pieces) {
+        const int4 piece = p.pieces[item];
+        i = piece.x;
+        rows = p.perm + piece.y;
+        total = piece.z;
+        slot = piece.w;
+        if (i < 0) return;
+    } else if (p.perm) {
         const int first = p.offs[i];
         total = p.offs[i + 1] - first;
         rows = p.perm + first;
@@ -749,7 +782,7 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
         total = p.N <= 64 ? rows_by_ballots<1>(p, i, own) : rows_by_ballots<4>(p, i, own);
     }
     total = __builtin_amdgcn_readfirstlane(total);
-    const float f = total ? scale[i] : 0.f;
+    const float f = slot >= 0 ? 1.f : total ? scale[i] : 0.f;
     f32x4 acc[RT][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -757,6 +790,7 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
         for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     const long long slab = (long long)p.N * a.ldp;
     const bool whole = k0 + 64 <= a.K;                 // no lane's columns reach behind the end
+    const bool inside = r0 + 16 * RT <= a.ldp;         // no rank behind a row of part
     const int stride = SPLIT ? 4 : 1, groups = (total + 15) >> 4;
     int n[4];                                          // this lane's rows of the next group
     auto find = [&](int group) {
@@ -772,18 +806,32 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
             if (whole) x[s] = load4(xp);
             else x[s] = k < a.K ? load4(xp, a.K - k) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const float *gp = a.part + (long long)n[s] * a.ldp;
-#pragma unroll
-            for (int t = 0; t < RT; ++t) g[s][t] = gp[r0 + 16 * t + j < R ? r0 + 16 * t + j : 0];
-        }
-        for (int sl = 1; sl < a.slices; ++sl)
+        if (inside) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float *gp = a.part + sl * slab + (long long)n[s] * a.ldp;
+                const float *gp = a.part + (long long)n[s] * a.ldp + r0 + j;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) g[s][t] += gp[r0 + 16 * t + j < R ? r0 + 16 * t + j : 0];
+                for (int t = 0; t < RT; ++t) g[s][t] = gp[16 * t];
+            }
+        } else {                                       // the caller's h: no ranks behind R to read
+#pragma unroll 1
+            for (int t = 0; t < RT; ++t) {
+                const int r = r0 + 16 * t + j < R ? r0 + 16 * t + j : 0;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const float v = a.part[(long long)n[s] * a.ldp + r];
+#pragma unroll
+                    for (int k = 0; k < RT; ++k) g[s][k] = k == t ? v : g[s][k];
+                }
+            }
+        }
+#pragma unroll 1
+        for (int sl = 1; sl < a.slices; ++sl)          // (only kernels' partial sums come in slices)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float *gp = a.part + sl * slab + (long long)n[s] * a.ldp + r0 + j;
+#pragma unroll
+                for (int t = 0; t < RT; ++t) g[s][t] += gp[16 * t];
             }
     };
     auto multiply = [&](f32x4(&x)[4], float(&g)[4][RT], int group) {
@@ -811,10 +859,11 @@ __device__ inline void rows_tile(const RowsArgs<T> &a, const Plan &p, const floa
         find(group + stride);
         multiply(x, g, group);
     }
-    float *out = a.out + i * a.so;
+    float *out = slot >= 0 ? a.apart + slot * (R * a.lda) : a.out + i * a.so;
+    const long long ldo = slot >= 0 ? a.lda : a.ldo;
     auto put = [&](int r, int c, f32x4 val) {
         if (r >= R || c >= a.K) return;
-        float *o = out + r * a.ldo + c;
+        float *o = out + r * ldo + c;
         if (a.K - c >= 4) *(f32x4_m *)o = f * val;
         else
             for (int y = 0; y < a.K - c; ++y) o[y] = f * val[y];
@@ -845,6 +894,33 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsArgs<T> a, const Ro
     else rows_tile<float, RT, SPLIT>(b, p, scale, R, blockIdx.x, red, own);          // (fewer: a long one last would be waited for)
 }
 
+// out[i] = scale[i] times the sum of the pieces of an adapter that has several, in order
+template <class T>
+__device__ inline void join_pieces(const RowsArgs<T> &a, int i, int slot, int n, float f, int R, long long first, long long step) {
+    const long long row4 = a.lda / 4;
+    for (long long e = first; e < R * row4; e += step) {
+        const int r = (int)(e / row4), c = 4 * (int)(e - r * row4);
+        const float *src = a.apart + (slot * (long long)R + r) * a.lda + c;
+        f32x4 v = *(const f32x4 *)src;
+#pragma unroll 4
+        for (int k = 1; k < n; ++k) v += *(const f32x4 *)(src + k * (R * a.lda));
+        float *o = a.out + i * a.so + r * a.ldo + c;
+        if (a.K - c >= 4) *(f32x4_m *)o = f * v;
+        else
+            for (int y = 0; y < a.K - c; ++y) o[y] = f * v[y];
+    }
+}
+template <class T>
+__global__ __launch_bounds__(256) void join_pieces_kernel(const RowsArgs<T> a, const RowsArgs<float> b, const int2 *__restrict__ slots,
+                                                          const float *__restrict__ scale, int R, int blocks) {
+    const int slot = blockIdx.x / blocks, k = blockIdx.x - slot * blocks;
+    const int2 s = slots[slot];                        // {adapter, its pieces: at the first of its slots alone}
+    if (s.y == 0) return;
+    const float f = scale[s.x];
+    join_pieces(a, s.x, slot, s.y, f, R, k * 256ll + threadIdx.x, blocks * 256ll);
+    join_pieces(b, s.x, slot, s.y, f, R, k * 256ll + threadIdx.x, blocks * 256ll);
+}
+
 // part[0] = sum_s part[s], in order: where so many slices were needed that every reader joining them would cost more
 __global__ __launch_bounds__(256) void join_kernel(float *part, long long n4, int slices) {
     f32x4 *p = (f32x4 *)part;
@@ -870,7 +946,9 @@ struct Layout {
     int rt, nt;                // ranks and rows of a tile, in 16s
     int max_tiles;
     bool sorted;               // plan_kernel's list, not each workgroup's own
-    size_t perm, offs, tiles, part, part2, bytes;
+    bool pieced;               // backward of a long batch: adapters in pieces of kPiece rows
+    int max_pieces, max_slots;
+    size_t perm, offs, tiles, pieces, slots, apart_a, apart_b, part, part2, bytes;
     int slices, slices2;       // K slices of the first contraction and, backward only, of the one that computes h again
 };
 
@@ -908,6 +986,18 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     y.perm = take(y.sorted ? 4 * (size_t)N : 0);
     y.offs = take(y.sorted ? 4 * ((size_t)L + 1) : 0);
     y.tiles = take(y.sorted ? 16 * (size_t)y.max_tiles : 0);
+    // Pieces from 2048 rows on: one adapter's rows then no longer hold up the rest.  Backward of 4096 rows x 12544: 64 adapters of
+    // rank 64, a fourth of the rows on one, 163 us in pieces, 305 whole; one adapter of rank 8 75 and 139; evenly over 64 adapters
+    // 210 and 206 (the launch that joins); 1024 rows of 4 adapters 39 and 34.
+    // At most one piece an adapter and one for every kPiece rows; slots only for adapters with more rows than that, so at most
+    // one for every kPiece / 2 rows.
+    y.pieced = back && N >= 2048;
+    y.max_pieces = y.pieced ? L + N / kPiece : 0;
+    y.max_slots = y.pieced ? N / (kPiece / 2) : 0;
+    y.pieces = take(16 * (size_t)y.max_pieces);
+    y.slots = take(8 * (size_t)y.max_slots);
+    y.apart_a = take(16 * (size_t)y.max_slots * R * ((K + 3ll) / 4));
+    y.apart_b = take(16 * (size_t)y.max_slots * R * ((U + 3ll) / 4));
     y.part = take(64 * (size_t)y.slices * N * y.rt);
     y.part2 = take(64 * (size_t)y.slices2 * N * y.rt);
     y.bytes = at < 256 ? 256 : at;
@@ -915,17 +1005,21 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
 }
 
 Plan make_plan(const Layout &y, char *ws, const int32_t *index, int N, int L, hipStream_t s) {
-    Plan p = {index, N, L, nullptr, nullptr, nullptr};
+    Plan p = {index, N, L, nullptr, nullptr, nullptr, nullptr};
     if (!y.sorted) return p;
     int waves = 15360 / (L + 1), bits = 1;             // 60 KB of counters
     waves = waves > 16 ? 16 : waves;
     while (1 << bits < L + 1) ++bits;
     int *perm = (int *)(ws + y.perm), *offs = (int *)(ws + y.offs);
-    int4 *tiles = (int4 *)(ws + y.tiles);
-    plan_kernel<<<dim3(1), dim3(1024), (size_t)waves * (L + 1) * 4, s>>>(index, N, L, waves, bits, 16 * y.nt, perm, offs, tiles, y.max_tiles);
+    int4 *tiles = (int4 *)(ws + y.tiles), *pieces = y.pieced ? (int4 *)(ws + y.pieces) : nullptr;
+    const size_t lds = (size_t)waves * (L + 1) * 4;
+#define CALL(PIECES) plan_kernel<PIECES><<<dim3(1), dim3(1024), lds, s>>>(index, N, L, waves, bits, 16 * y.nt, perm, offs, tiles, y.max_tiles, pieces, y.max_pieces, (int2 *)(ws + y.slots), y.max_slots)
+    if (y.pieced) CALL(true); else CALL(false);
+#undef CALL
     p.perm = perm;
     p.offs = offs;
     p.tiles = tiles;
+    p.pieces = pieces;
     return p;
 }
 
@@ -1030,16 +1124,17 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
                 ws_bytes, y.bytes);
     // Many rows to an adapter are split over the waves of a workgroup (rows_tile), unless the adapters fill the chip without it:
     // 500 rows of 8 adapters at rank 16 12 us split, 31 not; 2048 of 16 at rank 32 54 and 142; 4096 of 64 at rank 64 (the whole
-    // call) 224 split, 174 not; 600 rows of 20 adapters, fewer than 32 each, 37 split, 33 not.
-    const bool split = N > 32ll * (L < N ? L : N) && L * ((K + 255ll) / 256 + (U + 255ll) / 256) < 2048;
+    // call) 224 split, 174 not; 600 rows of 20 adapters, fewer than 32 each, 37 split, 33 not (measured without pieces).
+    const int items = y.pieced ? y.max_pieces : L;
+    const bool split = N > 32ll * (L < N ? L : N) && items * ((K + 255ll) / 256 + (U + 255ll) / 256) < 2048;
     const int wide = split ? 64 : 256;
     const long long ka = (K + wide - 1ll) / wide, ub = (U + wide - 1ll) / wide;
-    TY1_REQUIRE(2 * L * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
+    TY1_REQUIRE(2 * items * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
     if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 8 * ((K + 255ll) / 256)))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_backward", s, 2.0 * N * R * (K * (dx ? 2.0 : 1.0) + 2.0 * U),
                         sizeof(T) * (double)N * K + 4.0 * N * U + 4.0 * L * R * ((double)K + U) + (dx ? 4.0 * N * K : 0.0));
-    Plan p = {index, N, L, nullptr, nullptr, nullptr};
+    Plan p = {index, N, L, nullptr, nullptr, nullptr, nullptr};
     float *part = (float *)((char *)ws + y.part), *part2 = (float *)((char *)ws + y.part2);
     if (N > 0) {
         p = make_plan(y, (char *)ws, index, N, L, s);
@@ -1051,16 +1146,21 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
         }
     }
     const int ranks = y.rt == 8 ? 2 : 1;               // (128 ranks of accumulators would leave one wave a SIMD)
-    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, 16 * y.rt, (int)ka, ranks};
-    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, 1, h ? R : 16 * y.rt, (int)ub, ranks};
-    const dim3 grid((unsigned)(L * ranks * (ka + ub)));
+    const RowsArgs<T> ra = {part, x, da, ldx, ldda, sda, K, y.slices, 16 * y.rt, (int)ka, ranks, (float *)((char *)ws + y.apart_a), (K + 3ll) & ~3ll};
+    const RowsArgs<float> rb = {h ? h : part2, dz, db, lddz, lddb, sdb, U, 1, h ? R : 16 * y.rt, (int)ub, ranks, (float *)((char *)ws + y.apart_b), (U + 3ll) & ~3ll};
+    const dim3 grid((unsigned)(items * ranks * (ka + ub)));
 #define CALL(RT)                                                                                                                    \
     do {                                                                                                                            \
-        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ub));                          \
-        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(L * ranks * ub));                               \
+        if (split) rows_kernel<T, RT, true><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(items * ranks * ub));                          \
+        else rows_kernel<T, RT, false><<<grid, dim3(256), 0, s>>>(ra, rb, p, scale, R, (int)(items * ranks * ub));                               \
     } while (0)
     if (y.rt == 1) CALL(1); else if (y.rt == 2) CALL(2); else CALL(4);
 #undef CALL
+    if (y.pieced) {
+        const int each = 8192 / y.max_slots, blocks = each < 16 ? 16 : each > 256 ? 256 : each;
+        TY1_REQUIRE((long long)y.max_slots * blocks < (1ll << 24), "%s: %d rows are more than one launch holds", what, N);
+        join_pieces_kernel<T><<<dim3((unsigned)(y.max_slots * blocks)), dim3(256), 0, s>>>(ra, rb, (const int2 *)((char *)ws + y.slots), scale, R, blocks);
+    }
     if (dx && N > 0) expand<T>(y, p, part, y.slices, a, lda, sa, scale, dx, lddx, nullptr, K, R, 0, s);
     return ty1::check_launch(what);
 }
