@@ -117,12 +117,13 @@ LONG = [(4000, 9001, 33, 2, 64, torch.float32), (2100, 9003, 20, 1, 100, torch.f
         (4000, 9001, 35, 3, 9, torch.float32), (4000, 16500, 20, 2, 40, torch.bfloat16), (4000, 40, 9001, 2, 30, torch.bfloat16),
         (4000, 40, 9001, 2, 61, torch.bfloat16), (2100, 30, 9002, 1, 128, torch.bfloat16), (4000, 64, 4100, 2, 17, torch.float32),
         (40, 100, 50, 5, 100, torch.float32), (600, 20, 16, 4096, 3, torch.float32), (256, 40, 20, 4096, 2, torch.bfloat16),
-        (257, 513, 1025, 1, 1, torch.float32), (2049, 303, 77, 700, 5, torch.float32), (5000, 130, 61, 1500, 18, torch.bfloat16)]
+        (257, 513, 1025, 1, 1, torch.float32), (2049, 303, 77, 700, 5, torch.float32),
+        (701, 303, 77, 1, 16, torch.bfloat16), (5000, 130, 61, 1500, 18, torch.bfloat16)]
 
 
 def test_one_adapter_with_most_of_the_rows():
-    """Adapters of 0, 1, 256, 257, 512, 513 and the rest of 4000 rows: one piece, several, whole last ones and single rows."""
-    N, K, U, L, R = 4000, 301, 70, 8, 12
+    """Adapters of 0, 1, 256, 257, 512, 513 and the rest of 4200 rows: one piece, several, whole last ones and single rows."""
+    N, K, U, L, R = 4200, 301, 70, 8, 12
     x, a, b, _, scale, dz = _inputs(N, K, U, L, R, torch.float32, 12, whole=True)
     counts = [0, 1, 256, 257, 512, 513, N - 1 - 256 - 257 - 512 - 513 - 40]
     index = torch.cat([torch.full((c,), i) for i, c in enumerate(counts)] + [torch.full((40,), -1)])

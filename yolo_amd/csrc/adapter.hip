@@ -34,7 +34,7 @@ constexpr int kPiece = 256;               // rows of an adapter that one workgro
 // The rows of a batch come in any order of adapters; a tile is up to TM rows of ONE adapter, so that the adapter's weights are
 // read once for all of them.  Rows without an adapter (index < 0 or >= L) form a class of their own, L, whose tiles are only
 // filled in.  Up to kSelfPlan rows every workgroup works its tile out from the index itself; above, one workgroup sorts the
-// rows once (plan_kernel, 4 to 6 us and a launch) and the others read the list.
+// rows once (plan_kernel, 5 to 10 us and a launch) and the others read the list.
 struct Plan {
     const int *index;          // (N)
     int N, L;
@@ -986,12 +986,12 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     y.perm = take(y.sorted ? 4 * (size_t)N : 0);
     y.offs = take(y.sorted ? 4 * ((size_t)L + 1) : 0);
     y.tiles = take(y.sorted ? 16 * (size_t)y.max_tiles : 0);
-    // Pieces from 2048 rows on: one adapter's rows then no longer hold up the rest.  Backward of 4096 rows x 12544: 64 adapters of
-    // rank 64, a fourth of the rows on one, 163 us in pieces, 305 whole; one adapter of rank 8 75 and 139; evenly over 64 adapters
-    // 210 and 206 (the launch that joins); 1024 rows of 4 adapters 39 and 34.
-    // At most one piece an adapter and one for every kPiece rows; slots only for adapters with more rows than that, so at most
-    // one for every kPiece / 2 rows.
-    y.pieced = back && N >= 2048;
+    // Pieces where one adapter's rows would hold up the rest: from 700 rows an adapter on, and from 4096 rows whatever the mean (a
+    // batch can lean on one adapter).  Backward x 12544: one adapter, 2048 rows of rank 32 64 us in pieces, 91 whole; 1024 of rank
+    // 16 39 and 48; 2048 rows of 8 adapters 66 and 57; 4096 rows of 64 adapters of rank 64 210 and 206, with a fourth of them on
+    // one adapter 163 and 305 (539 units).  At most one piece an adapter and one for every kPiece rows; slots only for adapters
+    // with more rows than that, so at most one for every kPiece / 2 rows.
+    y.pieced = back && y.sorted && (N >= 700ll * classes || N >= 4096);
     y.max_pieces = y.pieced ? L + N / kPiece : 0;
     y.max_slots = y.pieced ? N / (kPiece / 2) : 0;
     y.pieces = take(16 * (size_t)y.max_pieces);
@@ -1130,6 +1130,8 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     const int wide = split ? 64 : 256;
     const long long ka = (K + wide - 1ll) / wide, ub = (U + wide - 1ll) / wide;
     TY1_REQUIRE(2 * items * (ka + ub) < (1ll << 24), "%s: %d adapters of %d x %d are more than one launch holds", what, L, K, U);
+    const int each = y.pieced ? 8192 / y.max_slots : 0, blocks = each < 16 ? 16 : each > 256 ? 256 : each;      // to a slot, in the joining launch
+    TY1_REQUIRE((long long)y.max_slots * blocks < (1ll << 24), "%s: %d rows are more than one launch holds", what, N);
     if (check_grid(what, y, y.slices) || check_grid(what, y, y.slices2) || (dx && check_grid(what, y, 8 * ((K + 255ll) / 256)))) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("adapter_backward", s, 2.0 * N * R * (K * (dx ? 2.0 : 1.0) + 2.0 * U),
@@ -1157,8 +1159,6 @@ int backward(const char *what, const float *dz, const T *x, const T *a, const T 
     if (y.rt == 1) CALL(1); else if (y.rt == 2) CALL(2); else CALL(4);
 #undef CALL
     if (y.pieced) {
-        const int each = 8192 / y.max_slots, blocks = each < 16 ? 16 : each > 256 ? 256 : each;
-        TY1_REQUIRE((long long)y.max_slots * blocks < (1ll << 24), "%s: %d rows are more than one launch holds", what, N);
         join_pieces_kernel<T><<<dim3((unsigned)(y.max_slots * blocks)), dim3(256), 0, s>>>(ra, rb, (const int2 *)((char *)ws + y.slots), scale, R, blocks);
     }
     if (dx && N > 0) expand<T>(y, p, part, y.slices, a, lda, sa, scale, dx, lddx, nullptr, K, R, 0, s);
