@@ -295,7 +295,7 @@ def test_nothing_to_do():
     assert int(da.count_nonzero()) == 0 and int(db.count_nonzero()) == 0 and dx.shape == (0, 20)
 
 
-@pytest.mark.parametrize('N', [500, 2500])
+@pytest.mark.parametrize('N', [500, 2500, 4500])
 def test_same_bits_every_time_and_apart_from_the_other_rows(N):
     """A run repeated gives the same bits; so does a row's result whatever rows stand beside it in the batch, as long as the
     batch takes the same variant (same N)."""
@@ -310,7 +310,7 @@ def test_same_bits_every_time_and_apart_from_the_other_rows(N):
     assert torch.equal(out, first[0][perm])
 
 
-@pytest.mark.parametrize('N', [80, 700])
+@pytest.mark.parametrize('N', [80, 700, 4200])
 def test_on_a_side_stream_and_in_graphs(N):
     """Two graphs captured one after the other, replayed in turn with eager work between, and calls on two streams at once:
     every result is the eager one."""
