@@ -284,7 +284,9 @@ int ty1_adam_step_f32(float *p, const float *g, float *m, float *v, int64_t n, f
  * scale (L) f32, out (N,U) f32 with row stride ldo, h (N,R) f32 or NULL: kept for the backward pass (without scale).  All
  * sums are float32.  1 <= R <= 128, 1 <= L <= 4096, N, K, U up to 2^30; a smaller rank is padded with zero rows of A and B.
  * out and h must not overlap the operands or one another (nor da, db, dx below).
- * workspace: scratch of ty1_adapter_workspace_bytes() bytes, 16-byte aligned, for this call alone.  Laid out as one more split of ty1_dense_splitk_f32's partials, out is summed by whatever kernel reduces those.
+ * workspace: scratch of ty1_adapter_workspace_bytes() bytes, 16-byte aligned, for this call alone.
+ * With out = the last of ty1_dense_splitk_*'s partials and accumulate, whatever kernel reduces those adds the adapters on the
+ * way, and rows without an adapter keep their bits (one partial more would change the order of every row's sum).
  */
 int ty1_adapter_workspace_bytes(int N, int K, int U, int L, int R, int backward, size_t *bytes);
 int ty1_adapter_forward_f32(const float *x, const float *a, const float *b, const int32_t *index, const float *scale,

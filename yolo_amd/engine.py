@@ -101,7 +101,8 @@ class DeviceModel:
     def dense(self, feats, ws=None, adapters=None, index=None, h=None):
         """Split-K partials (splits,N,ldz) of the Dense layer for the kernels behind it.  adapters (adapters.AdapterBank) and
         index (N) int32 on the device (AdapterBank.index; -1: none): image n goes through the Dense layer plus adapter index[n],
-        whose product is one more partial, summed by whatever kernel reduces the others.  h: see ops.adapter_forward."""
+        whose product is added to the last partial.  (As a partial of its own it would change the order in which the kernels
+        behind sum the others, and with it the bits of the images without an adapter.)  h: see ops.adapter_forward."""
         ws = ws or self.workspace(feats.shape[0])
         wt = self.dense_wt_bf16 if self.dtype == 'bf16' else self.dense_wt
         if adapters is None:
@@ -112,13 +113,9 @@ class DeviceModel:
             raise ValueError('adapters need an index: one adapter per image, -1 for none')
         if (adapters.features, adapters.units) != (self.K, self.units):
             raise ValueError(f'adapters of a {adapters.features} x {adapters.units} Dense layer do not fit {self.K} x {self.units}')
-        part = ws.get('part_adapted')
-        if part is None:
-            splits, N, ldz = ws['part'].shape
-            part = ws['part_adapted'] = torch.empty((splits + 1, N, ldz), dtype=torch.float32, device=self.device)
-        ops.dense_splitk(feats, wt, self.units, part=part[:-1])
         a, b = adapters.weights(feats.dtype)
-        ops.adapter_forward(feats, a, b, index, adapters.scale, out=part[-1][:, :self.units], h=h)
+        part = ops.dense_splitk(feats, wt, self.units, part=ws['part'])
+        ops.adapter_forward(feats, a, b, index, adapters.scale, out=part[-1][:, :self.units], accumulate=True, h=h)
         return part
 
     def head(self, feats, ws=None, adapters=None, index=None):

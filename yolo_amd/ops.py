@@ -566,8 +566,8 @@ def adapter_forward(x, a, b, index, scale, out=None, accumulate=False, h=None):
     repeated by expand); index (N) int32; scale (L) float32 -> out (N,U) float32, sums in float32.
     index[n] < 0: no adapter for this row (zeros).  index[n] >= L: the row becomes NaN (the index lives on the GPU and is not
     read by the host).  Smaller ranks: zero rows in a and b.
-    out: where to write, e.g. part[splits][:, :U] behind the partials of dense_splitk - the kernel that reduces those then adds
-    the adapters at no cost.  accumulate: add to what out holds instead (rows without an adapter stay as they are).
+    out: where to write.  accumulate: add to what out holds instead (rows without an adapter stay as they are), e.g. to
+    part[-1][:, :U], the last of dense_splitk's partials: whatever kernel reduces those then adds the adapters on the way.
     h: optional (N,R) float32 that receives x . a^T (without scale) for adapter_backward."""
     dev, N, K, U, L, R = _adapter_operands(x, a, b, index, scale)
     if out is None:
