@@ -328,7 +328,8 @@ int ty1_adapter_backward_bf16(const float *dz, const void *x, const void *a, con
  * grads, outs, p, g, m, v, counts and dtypes are HOST arrays of n entries: device pointers (aligned to their type), numbers
  * of values, and TY1_F32 or TY1_BF16 (dtypes NULL: all float32).  norm (1) f32 on the device.  Nothing of the host arrays is
  * read after the call returns.  A tensor that is written must not overlap any other tensor of the call, except outs[t] with
- * grads[t] of the same t and address (refused).  max_norm > 0, infinity included.  1 - beta1, 1 - beta2 and the bias-corrected
+ * grads[t] of the same t and address (refused).  workspace: ty1_grad_norm_workspace_bytes(n) bytes, aligned to 8, apart from every
+ * tensor and the norm (refused).  max_norm > 0, infinity included.  1 - beta1, 1 - beta2 and the bias-corrected
  * rate are taken in float64 and rounded once.
  */
 enum { TY1_F32 = 0, TY1_BF16 = 1 };

@@ -274,6 +274,24 @@ int check_overlap(const char *what, int n, const int64_t *counts, const int *dty
     return 0;
 }
 
+size_t partials(int n) { return ((size_t)n + kTensors - 1) / kTensors * kBlocks; }
+
+// The norm and the scratch memory: alignments, and no partial sum may be written over a value that is still to be read.
+int check_scratch(const char *what, int n, const int64_t *counts, const int *dtypes, void *const *const *lists, int n_lists,
+                  const float *norm, const void *ws, size_t ws_bytes) {
+    const size_t need = partials(n) * sizeof(double);
+    TY1_REQUIRE(norm && ws && ws_bytes >= need, "%s: null pointer or workspace too small", what);
+    TY1_REQUIRE(((uintptr_t)norm & 3) == 0 && ((uintptr_t)ws & 7) == 0, "%s: norm not aligned to 4 bytes or workspace not aligned to 8", what);
+    const uintptr_t lo = (uintptr_t)ws, hi = lo + need, at = (uintptr_t)norm;
+    TY1_REQUIRE(at + 4 <= lo || at >= hi, "%s: the workspace shares memory with the norm", what);
+    for (int l = 0; l < n_lists; ++l)
+        for (int t = 0; t < n; ++t) {
+            const uintptr_t a = (uintptr_t)lists[l][t], b = a + (uintptr_t)counts[t] * (dtypes && dtypes[t] == TY1_BF16 ? 2 : 4);
+            TY1_REQUIRE(counts[t] == 0 || b <= lo || a >= hi, "%s: the workspace shares memory with tensor %d", what, t);
+        }
+    return 0;
+}
+
 // lists of n host pointers: element sizes and addresses have to fit
 int check_lists(const char *what, int n, const int64_t *counts, const int *dtypes, void *const *const *lists, int n_lists) {
     TY1_REQUIRE(n >= 1 && counts, "%s: no tensors", what);
@@ -312,8 +330,6 @@ bool fill_small(Lists &ls, int n, const int64_t *counts, const int *dtypes, void
     return fill(ls, 0, n, counts, dtypes, lists, n_lists) == n && ls.start[ls.n] <= limit;
 }
 
-size_t partials(int n) { return (size_t)((n + kTensors - 1) / kTensors) * kBlocks; }
-
 // the squares of one list, launch by launch -> number of partial sums in ws
 int launch_norm(int n, const int64_t *counts, const int *dtypes, void *const *list, double *part, hipStream_t s) {
     int parts = 0;
@@ -339,7 +355,7 @@ extern "C" int ty1_grad_norm_workspace_bytes(int n, size_t *bytes) {
 extern "C" int ty1_grad_norm(void *const *grads, const int64_t *counts, const int *dtypes, int n, float *norm, void *workspace,
                              size_t workspace_bytes, ty1_stream_t stream) {
     if (check_lists("ty1_grad_norm", n, counts, dtypes, &grads, 1)) return 1;
-    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_grad_norm: null pointer or workspace too small");
+    if (check_scratch("ty1_grad_norm", n, counts, dtypes, &grads, 1, norm, workspace, workspace_bytes)) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("grad_norm", s);
     Lists ls;
@@ -357,7 +373,7 @@ extern "C" int ty1_clip_grad_norm(void *const *grads, void *const *outs, const i
     void *const *lists[2] = {grads, outs};
     if (check_lists("ty1_clip_grad_norm", n, counts, dtypes, lists, 2)) return 1;
     TY1_REQUIRE(max_norm > 0.0, "ty1_clip_grad_norm: max_norm=%g must be positive", max_norm);
-    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_clip_grad_norm: null pointer or workspace too small");
+    if (check_scratch("ty1_clip_grad_norm", n, counts, dtypes, lists, 2, norm, workspace, workspace_bytes)) return 1;
     if (check_overlap("ty1_clip_grad_norm", n, counts, dtypes, lists, 2, 2u, true, norm)) return 1;
     hipStream_t s = (hipStream_t)stream;
     ty1::ProfScope prof("clip_grad_norm", s);
@@ -383,7 +399,7 @@ extern "C" int ty1_adam_step_clip_f32(void *const *p, void *const *g, void *cons
     TY1_REQUIRE(max_norm > 0.0, "ty1_adam_step_clip: max_norm=%g must be positive", max_norm);
     TY1_REQUIRE(t >= 1, "ty1_adam_step_clip: bad t=%lld", (long long)t);
     TY1_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "ty1_adam_step_clip: betas %g, %g must lie in [0, 1)", beta1, beta2);
-    TY1_REQUIRE(norm && workspace && workspace_bytes >= partials(n) * sizeof(double), "ty1_adam_step_clip: null pointer or workspace too small");
+    if (check_scratch("ty1_adam_step_clip", n, counts, nullptr, lists, 4, norm, workspace, workspace_bytes)) return 1;
     if (check_overlap("ty1_adam_step_clip", n, counts, nullptr, lists, 4, 13u, false, norm)) return 1;
     const double lr_t = lr * std::sqrt(1.0 - std::pow(beta2, (double)t)) / (1.0 - std::pow(beta1, (double)t));
     hipStream_t s = (hipStream_t)stream;
