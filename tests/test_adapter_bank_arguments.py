@@ -1,0 +1,35 @@
+"""CPU: what an AdapterBank refuses, and that a refused call leaves the bank as it was."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from yolo_amd.adapters import AdapterBank
+
+
+def _bank():
+    return AdapterBank(types.SimpleNamespace(K=50, units=13, device=torch.device('cpu')), 3, 4)
+
+
+@pytest.mark.parametrize('which', [[True, False], [0, False], np.array([True, False]), torch.tensor([False, True]), [np.True_, 0]])
+def test_a_mask_is_not_a_list_of_adapters(which):
+    with pytest.raises(ValueError, match='adapter'):
+        _bank().index(which)
+
+
+@pytest.mark.parametrize('i', [1.5, -0.5, True, '1', None, np.float32(1), torch.tensor(0.5)])
+def test_an_adapter_number_is_whole(i):
+    bank = _bank()
+    with pytest.raises((TypeError, IndexError)):
+        bank.get(i)
+    with pytest.raises((TypeError, IndexError)):
+        bank.set(i, np.ones((2, 50)), np.ones((2, 13)))
+
+
+@pytest.mark.parametrize('i', [2, np.int64(2), np.int32(2), torch.tensor(2)])
+def test_whole_numbers_of_any_kind(i):
+    bank = _bank()
+    bank.set(i, np.ones((2, 50)), np.ones((2, 13)))
+    assert bool((bank.get(i)[1][:2] == 1).all()) and int(bank.b[:2].count_nonzero()) == 0
+    assert bank.index([int(i), -1]).tolist() == [2, -1]

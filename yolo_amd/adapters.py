@@ -4,6 +4,8 @@ The Dense layer is the only trainable layer of the network (/root/reference/mode
 BatchNormalization layer is frozen), so a detector fine-tuned for one camera or customer differs from the shared one in 73.8 MB
 of weights.  An adapter keeps that difference as W + scale * B^T A of rank R (0.9 MB at rank 16), and one batch may hold images
 of any mixture of adapters.  The reference has one set of weights and no counterpart."""
+import operator
+
 import numpy as np
 import torch
 
@@ -57,14 +59,16 @@ class AdapterBank:
         """Adapter numbers on the host, one per image (-1 or None: the shared weights alone) -> checked int32 tensor on the GPU."""
         which = [-1 if w is None else w for w in (which.tolist() if hasattr(which, 'tolist') else which)]
         for w in which:
-            if not isinstance(w, (int, np.integer)) or not -1 <= w < self.count:
+            if not isinstance(w, (int, np.integer)) or isinstance(w, bool) or not -1 <= w < self.count:
                 raise ValueError(f'adapter {w!r}: expected -1 (none) or 0 to {self.count - 1}')
         return torch.tensor(which, dtype=torch.int32).to(self.device)
 
     def _check(self, i):
-        if not 0 <= int(i) < self.count:
+        if isinstance(i, bool):
+            raise TypeError(f'adapter {i}: expected a number')
+        if not 0 <= operator.index(i) < self.count:
             raise IndexError(f'adapter {i}: the bank has {self.count}')
-        return int(i)
+        return operator.index(i)
 
     def set(self, i, a, b, scale=None):
         """Store one adapter from host arrays: a (r, features), b (r, units) with r <= rank (the ranks behind r become zero)."""
