@@ -33,3 +33,13 @@ def test_whole_numbers_of_any_kind(i):
     bank.set(i, np.ones((2, 50)), np.ones((2, 13)))
     assert bool((bank.get(i)[1][:2] == 1).all()) and int(bank.b[:2].count_nonzero()) == 0
     assert bank.index([int(i), -1]).tolist() == [2, -1]
+
+
+@pytest.mark.parametrize('scale', ['high', [1.0, 2.0], object()])
+def test_a_refused_scale_leaves_the_adapter_as_it_was(scale):
+    bank = _bank()
+    bank.set(1, np.full((4, 50), 3.0), np.full((4, 13), 4.0), scale=0.5)
+    with pytest.raises((TypeError, ValueError)):
+        bank.set(1, np.ones((2, 50)), np.ones((2, 13)), scale=scale)
+    a, b, s = bank.get(1)
+    assert (a == 3).all() and (b == 4).all() and s == 0.5

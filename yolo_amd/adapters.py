@@ -72,7 +72,7 @@ class AdapterBank:
 
     def set(self, i, a, b, scale=None):
         """Store one adapter from host arrays: a (r, features), b (r, units) with r <= rank (the ranks behind r become zero)."""
-        i = self._check(i)
+        i, scale = self._check(i), None if scale is None else float(scale)
         a, b = (torch.as_tensor(np.ascontiguousarray(v, np.float32)) for v in (a, b))
         r = a.shape[0]
         if a.dim() != 2 or r > self.rank or tuple(a.shape) != (r, self.features) or tuple(b.shape) != (r, self.units):
@@ -80,7 +80,7 @@ class AdapterBank:
         self.a[i].zero_(); self.b[i].zero_()
         self.a[i, :r].copy_(a); self.b[i, :r].copy_(b)
         if scale is not None:
-            self.scale[i] = float(scale)
+            self.scale[i] = scale
         self.changed()
 
     def get(self, i):
