@@ -43,3 +43,31 @@ def test_a_refused_scale_leaves_the_adapter_as_it_was(scale):
         bank.set(1, np.ones((2, 50)), np.ones((2, 13)), scale=scale)
     a, b, s = bank.get(1)
     assert (a == 3).all() and (b == 4).all() and s == 0.5
+
+
+def test_the_bf16_copy_is_made_on_the_banks_device(monkeypatch):
+    """changed() while another GPU is the current one: the cast, and the wait for it, belong to the bank's device (recorded here
+    without one)."""
+    from yolo_amd import ops
+    bank, at, seen = _bank(), ['cuda:0'], []
+    bank.device, bank._bf16 = torch.device('cuda:1'), torch.zeros_like(bank.flat, dtype=torch.bfloat16)
+
+    class Device:
+        def __init__(self, device):
+            self.device = str(device)
+
+        def __enter__(self):
+            at.append(self.device)
+
+        def __exit__(self, *error):
+            at.pop()
+
+    def stream(device=None):
+        device = at[-1] if device is None else str(device)
+        return types.SimpleNamespace(synchronize=lambda: seen.append(('wait', device)))
+
+    monkeypatch.setattr(torch.cuda, 'device', Device)
+    monkeypatch.setattr(torch.cuda, 'current_stream', stream)
+    monkeypatch.setattr(ops, 'cast_bf16', lambda x, out: seen.append(('cast', at[-1])))
+    bank.changed()
+    assert seen == [('cast', 'cuda:1'), ('wait', 'cuda:1')] and at == ['cuda:0']

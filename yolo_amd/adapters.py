@@ -44,8 +44,9 @@ class AdapterBank:
         """a or b were written to: bring the bf16 copy of a bf16 model's bank up to date, in place, and wait for it (any stream may
         read it next, and graphs that were captured with it read the new values)."""
         if self._bf16 is not None:
-            ops.cast_bf16(self.flat, out=self._bf16)
-            torch.cuda.current_stream(self.device).synchronize()
+            with torch.cuda.device(self.device):       # (the cast goes to the current device's stream)
+                ops.cast_bf16(self.flat, out=self._bf16)
+                torch.cuda.current_stream().synchronize()
 
     def weights(self, dtype):
         """(a, b) for products in torch.float32 or, in a bf16 model's bank, torch.bfloat16."""
