@@ -240,13 +240,14 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int *__restrict__ inde
 //            holds 16 consecutive bytes of row j at q * 16 bytes - four steps of v_mfma_f32_16x16x4_f32 with k in another
 //            order, the same on both sides, or one of v_mfma_f32_16x16x32_bf16.  No barrier before the end: the shortest way
 //            for one slice (one row x 12544 of rank 8: 4.5 us, most of it launch and three dependent loads; 64 rows of 16
-//            adapters of rank 16, 16 MB: 7.5 us).
+//            adapters of rank 16, 16 MB: 7.1 to 8.2 us).
 //   staged   A fragment load is 64 cache accesses an instruction (its neighbouring lanes are different rows), which is what
 //            bounds the direct form in the long run.  Here 256 consecutive bytes of every row go through registers into
 //            LDS, 16 accesses an instruction, and the fragments are read from there.  A row's 16-byte pieces are permuted by
 //            its number: the 16 rows of a fragment read lie in 16 different bank groups.  The loads of the next stage are in
 //            flight while the present one multiplies (a second LDS buffer and 512-byte stages measured slower).  4096 rows
-//            x 12544 of 64 adapters of rank 64 in float32: 104 us, 447 MB fetched = 4.3 TB/s, matrix pipe half busy.
+//            x 12544 of 64 adapters of rank 64 in float32: 105 to 109 us, 436 MB read = 4.1 TB/s, matrix pipe 44 % busy
+//            (counters: profiles/adapters_clip_kernels.csv).
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) Piece_m {               // 16 bytes from wherever a row's elements lie
     u32x4 v;
@@ -344,7 +345,7 @@ __device__ inline void contract_direct(const ContractArgs<TX, TW> &a, const int 
     typedef Frag<TX, TW> F;
     typedef typename F::VX VX;
     typedef typename F::VM VM;
-    constexpr int R16 = 16 * RT, E = F::E, KC = 4 * E;
+    constexpr int E = F::E, KC = 4 * E;
     constexpr int UN = NT + RT >= 6 ? 2 : 16 / (NT + RT) > 4 ? 4 : 16 / (NT + RT);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
     const int chunks = a.K / KC;                       // whole fragments; the last slice also takes what is left of K
@@ -558,8 +559,9 @@ __global__ __launch_bounds__(256, 2) void contract_kernel(const ContractArgs<TX,
 // out[n][u] (+)= sum_r h[n][r] m[i][r][u] with h = scale[i] sum_s part[s]: one wave per 64 columns, lane (j, q) holding four
 // consecutive ones, so that loads of m and stores of out are 256 bytes a row.  Bound by reading m and writing out.  h is
 // joined from the K slices on the way (and stored, without the scale, where the caller keeps it).  float32 matrix instruction
-// for both types: bf16 weights are widened, h is not rounded.  One row x 1470: 5.4 us; 4096 rows x 539 of rank 64: 20 us; the
-// gradient of x of 2048 rows x 12544 of rank 32: 39 us, 167 MB moved = 4.3 TB/s.
+// for both types: bf16 weights are widened, h is not rounded.  One row x 1470: 5.3 us; 4096 rows x 539 of rank 64: 20.5 us, 49 MB
+// moved, the K slices read again by every column block among them; the gradient of x of 2048 rows x 12544 of rank 32: 39 us, 131 MB
+// moved = 3.3 TB/s (counters: profiles/adapters_clip_kernels.csv).
 __device__ inline f32x4 load4(const float *p) { return *(const f32x4_m *)p; }
 __device__ inline f32x4 load4(const bf16 *p) {
     const bf16x4_m v = *(const bf16x4_m *)p;
@@ -637,7 +639,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_ker
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, q = lane >> 4;
     // Workgroups that read the same part of m belong on one XCD (blockIdx % 8), whose L2 then fetches it once: the tiles of an
     // adapter on the same columns where there are 8 column blocks or more, the row blocks of a tile below that (gradient of x
-    // at 2048 rows x 12544: 39 -> 38 us; 4096 rows x 539 of rank 64: 24 -> 22.5).
+    // at 2048 rows x 12544: 39 -> 38 us; 4096 rows x 539 of rank 64: 24 -> 22.5, before the ranks came 16 at a time).
     int t, sub, block;
     if (a.blocks >= 8) {
         const int b8 = (a.blocks + 7) & ~7, ts = blockIdx.x / b8;
@@ -725,7 +727,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 4 : RT <= 2 ? 3 : 1) void expand_ker
 // out[i][r][k] = scale[i] sum over the rows n of adapter i of g[n][r] x[n][k], g = sum_s part[s]: lane (j, q) of a wave holds
 // four consecutive columns of row 4 step + q, so that loads of x and stores of out are 256 bytes a row.  Bound by reading x
 // and writing out once.  A wave runs through the adapter's rows by itself, 16 at a time, reading g from L2: a version that put
-// g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of 16 adapters of rank 32: 81 us, now 43 to 54).
+// g into LDS for the workgroup stood still at its barriers (2048 rows x 12544 of 16 adapters of rank 32: 81 us, now 44 to 56: 154 MB moved).
 // Two such products (A's gradient and B's) share a launch.  Loading the next 16 rows ahead costs more registers than it hides
 // latency (74 us): occupancy carries it.
 //   few rows to an adapter: a wave has 64 columns and all rows of the adapter or piece, a workgroup 256 columns;
@@ -990,7 +992,9 @@ Layout layout(int N, int K, int U, int L, int R, bool back) {
     // batch can lean on one adapter).  Backward x 12544: one adapter, 2048 rows of rank 32 64 us in pieces, 91 whole; 1024 of rank
     // 16 39 and 48; 2048 rows of 8 adapters 66 and 57; 4096 rows of 64 adapters of rank 64 210 and 206, with a fourth of them on
     // one adapter 163 and 305 (539 units).  At most one piece an adapter and one for every kPiece rows; slots only for adapters
-    // with more rows than that, so at most one for every kPiece / 2 rows.
+    // with more rows than that, so at most one for every kPiece / 2 rows (memory is reserved for all of them).  The host does not see
+    // the index: of 64 adapters of rank 64, a fourth of the rows on one, h kept and no dx, 4095 rows take 250 us whole and 4096 take 158
+    // in pieces, where rows spread evenly take 154 and 156.
     y.pieced = back && y.sorted && (N >= 700ll * classes || N >= 4096);
     y.max_pieces = y.pieced ? L + N / kPiece : 0;
     y.max_slots = y.pieced ? N / (kPiece / 2) : 0;

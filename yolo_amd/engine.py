@@ -516,7 +516,8 @@ class AdapterTrainer:
     all adapters where global_clipnorm is given.  The loss is the batch sum of yolo_loss (/root/reference/yolo/yolo.py:48-107)
     and data parallelism exchanges one flat buffer [dA | dB | loss] by SUM, as Trainer does.  Adapters without images in a step
     get a zero gradient; their moments decay and may still move them, as Keras' dense Adam does.  Everything runs in order on
-    the caller's stream."""
+    the caller's stream, in the model's buffers of this batch size: an update that a Trainer of the same model left in flight must be
+    joined first (Trainer.join())."""
 
     def __init__(self, model, bank, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-7, group=None, global_clipnorm=None):
         if model.dtype != 'f32':
